@@ -11,14 +11,20 @@ from .capi import (  # noqa: F401
     Sampler,
     apply_presence_penalty,
     apply_repetition_penalty,
+    beam_reorder,
+    beam_select,
     greedy_sample,
+    lmhead_logits_i8,
     load_library,
     make_params,
+    matmul_i8,
+    quantize_rows_i8,
     sample_batch,
     version,
 )
 
 __all__ = [
     "capi", "DllmError", "Sampler", "apply_presence_penalty", "apply_repetition_penalty",
-    "greedy_sample", "load_library", "make_params", "sample_batch", "version",
+    "beam_reorder", "beam_select", "greedy_sample", "lmhead_logits_i8", "load_library", "make_params",
+    "matmul_i8", "quantize_rows_i8", "sample_batch", "version",
 ]

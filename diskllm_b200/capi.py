@@ -24,6 +24,8 @@ STATUS_NAMES = {0: "OK", 1: "INVALID_ARG", 2: "OOM", 3: "CUDA", 4: "NCCL", 5: "T
                 6: "UNSUPPORTED"}
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+DTYPE_F16 = 2  # output weights, the int8 and the beam calls
+BEAM_MAX, BEAM_K_MAX = 128, 256
 MODE_TOPP_SORTED = 0x1
 MODE_PEN_TRUE_DIV = 0x2
 MODE_MINP_RELATIVE = 0x4
@@ -40,6 +42,9 @@ EXPORTS = [
     "dllm_cuda_set_debug_counters", "dllm_cuda_workspace_bytes", "dllm_cuda_sample_batch_static",
     "dllm_cuda_set_timing_events", "dllm_cuda_shard_candidates", "dllm_cuda_merge_sample",
     "dllm_cuda_append_history", "dllm_cuda_lmhead_logits",
+    "dllm_cuda_quantize_rows_i8", "dllm_cuda_matmul_i8", "dllm_cuda_lmhead_logits_i8",
+    "dllm_cuda_lmhead_i8_workspace_bytes", "dllm_cuda_beam_select", "dllm_cuda_beam_workspace_bytes",
+    "dllm_cuda_beam_reorder",
     "dllm_cuda_debug_inject_wait_timeout", "dllm_cuda_debug_fail_allocations",
     "dllm_cuda_peer_exchange_create", "dllm_cuda_peer_exchange_open", "dllm_cuda_peer_exchange_close",
     "dllm_cuda_peer_exchange_free", "dllm_cuda_shard_candidates_peer", "dllm_cuda_merge_sample_peer",
@@ -112,6 +117,34 @@ class BatchDesc(C.Structure):
     ]
 
 
+class BeamDesc(C.Structure):
+    """dllm_beam_desc"""
+    _fields_ = [
+        ("batch", C.c_int),
+        ("beams", C.c_int),
+        ("vocab", C.c_int),
+        ("k", C.c_int),
+        ("row_stride", C.c_int64),
+        ("dtype", C.c_int),
+        ("logits", C.c_void_p),
+        ("mask", C.c_void_p),
+        ("mask_stride", C.c_int64),
+        ("scores", C.c_void_p),
+        ("finished", C.c_void_p),
+        ("eos", C.c_int),
+        ("lengths", C.c_void_p),
+        ("length_penalty", C.c_float),
+        ("out_score", C.c_void_p),
+        ("out_parent", C.c_void_p),
+        ("out_token", C.c_void_p),
+        ("out_finished", C.c_void_p),
+        ("out_lengths", C.c_void_p),
+        ("status", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+    ]
+
+
 _lib = None
 
 
@@ -159,6 +192,21 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         f = getattr(lib, name)
         f.restype = C.c_int
         f.argtypes = args
+    i32, i64, f32, ptr = C.c_int, C.c_int64, C.c_float, C.c_void_p
+    for name, args in (("dllm_cuda_quantize_rows_i8", [i32, i32, ptr, i64, i32, i32, ptr, f32, i32, ptr, i64, ptr, ptr]),
+                       ("dllm_cuda_matmul_i8", [i32, i32, i32, ptr, i64, ptr, ptr, i64, ptr, f32, ptr, i64, i32, ptr,
+                                                ptr]),
+                       ("dllm_cuda_lmhead_logits_i8", [i32, i32, i32, ptr, ptr, f32, i32, ptr, i64, ptr, f32, ptr, ptr,
+                                                       ptr, C.c_size_t, ptr]),
+                       ("dllm_cuda_beam_select", [C.POINTER(BeamDesc), ptr]),
+                       ("dllm_cuda_beam_reorder", [i32, i32, ptr, i32, ptr, i64, i32, i64, i64, ptr])):
+        f = getattr(lib, name)
+        f.restype = C.c_int
+        f.argtypes = args
+    lib.dllm_cuda_lmhead_i8_workspace_bytes.restype = C.c_size_t
+    lib.dllm_cuda_lmhead_i8_workspace_bytes.argtypes = [i32, i32]
+    lib.dllm_cuda_beam_workspace_bytes.restype = C.c_size_t
+    lib.dllm_cuda_beam_workspace_bytes.argtypes = [C.POINTER(BeamDesc)]
     lib.dllm_cuda_workspace_bytes.restype = C.c_size_t
     lib.dllm_cuda_workspace_bytes.argtypes = [C.POINTER(BatchDesc)]
     lib.dllm_cuda_version.restype = C.c_char_p
@@ -635,3 +683,240 @@ def lmhead_logits(h, w, *, norm_w=None, eps=1e-6, add_one=False, softcap=0.0, lo
         raise DllmError(f"dllm_cuda_lmhead_logits: {STATUS_NAMES.get(rc, rc)} "
                         f"({load_library().dllm_cuda_last_error().decode()})")
     return logits
+
+
+# ---- int8 LM head -----------------------------------------------------------------------------
+
+_FLOATS = None
+
+
+def _float_code(dtype):
+    """DTYPE_* of a torch dtype, None for others."""
+    global _FLOATS
+    if _FLOATS is None:
+        import torch
+
+        _FLOATS = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
+    return _FLOATS.get(dtype)
+
+
+def _need(ok, what):
+    if not ok:
+        raise DllmError(what)
+
+
+def _vector(t, n, dtype, dev, name):
+    """A contiguous device vector of n elements."""
+    _need(t.dtype == dtype and t.device == dev and t.is_contiguous() and t.numel() == n,
+          f"{name}: a contiguous {dtype} tensor of {n} elements on {dev} is needed")
+    return t.data_ptr()
+
+
+def _codes(t, dev, name):
+    """(pointer, rows, cols, stride) of int8 rows that start on multiples of 16 bytes."""
+    import torch
+
+    _need(t.dtype == torch.int8 and t.device == dev and t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] <= 1),
+          f"{name}: int8 rows on {dev} are needed")
+    rows, cols = t.shape
+    stride = t.stride(0)
+    if rows <= 1:  # the stride of a single row is not used
+        stride = (cols + 15) // 16 * 16
+    _need(t.data_ptr() % 16 == 0 and stride % 16 == 0 and stride >= cols,
+          f"{name}: rows have to start on multiples of 16 bytes (quantize_rows_i8 lays them out so)")
+    return t.data_ptr(), rows, cols, stride
+
+
+def _call(name, dev, stream, *args):
+    """Runs a library call on `stream` (default: the current one of `dev`), with `dev` current."""
+    import torch
+
+    if stream is None:
+        stream = torch.cuda.current_stream(dev).cuda_stream
+    f = getattr(load_library(), name)
+    if torch.cuda.current_device() == dev.index:
+        _check(f(*args, stream), name)
+    else:
+        with torch.cuda.device(dev):
+            _check(f(*args, stream), name)
+
+
+def quantize_rows_i8(x, *, norm=False, norm_w=None, eps=1e-6, add_one=False, q=None, scale=None, stream=None):
+    """Rows to int8 codes with a scale each (dllm_cuda_quantize_rows_i8): x [rows][cols] fp32 / bf16 /
+    fp16, RMS-normalised first when `norm`.  Returns (codes int8 [rows][cols], scale fp32 [rows]); the
+    codes' rows start on multiples of 16 bytes."""
+    import torch
+
+    code = _float_code(x.dtype)
+    _need(x.is_cuda and x.dim() == 2 and code is not None, "x: a 2-D fp32, bf16 or fp16 CUDA tensor is needed")
+    rows, cols = x.shape
+    _need(cols >= 1 and (x.stride(1) == 1 or cols == 1), "x: rows of at least one element, contiguous")
+    dev = x.device
+    if q is None:
+        q = torch.empty(rows, (cols + 15) // 16 * 16, dtype=torch.int8, device=dev)[:, :cols]
+    if scale is None:
+        scale = torch.empty(rows, dtype=torch.float32, device=dev)
+    qp, qr, qc, qs = _codes(q, dev, "q")
+    _need((qr, qc) == (rows, cols), "q: the shape of x is needed")
+    wp = None if norm_w is None else _vector(norm_w, cols, torch.float32, dev, "norm_w")
+    _call("dllm_cuda_quantize_rows_i8", dev, stream, rows, cols, x.data_ptr(), max(x.stride(0), cols) if rows <= 1 else
+          x.stride(0), code, int(bool(norm)), wp, float(eps), int(bool(add_one)), qp, qs,
+          _vector(scale, rows, torch.float32, dev, "scale"))
+    return q, scale
+
+
+def matmul_i8(a, a_scale, b, b_scale, *, softcap=0.0, out=None, out_dtype=None, status=None, stream=None):
+    """out[i][j] = a_scale[i] b_scale[j] sum_k a[i][k] b[j][k] (dllm_cuda_matmul_i8): int8 codes a
+    [m][k], b [n][k] as quantize_rows_i8 gives them, fp32 scales; out fp32 (default), bf16 or fp16."""
+    import torch
+
+    _need(a.is_cuda, "a: a CUDA tensor is needed")
+    dev = a.device
+    ap, m, k, lda = _codes(a, dev, "a")
+    bp, n, kb, ldb = _codes(b, dev, "b")
+    _need(k == kb, f"a has {k} columns, b {kb}")
+    if out is None:
+        out = torch.empty(m, n, dtype=out_dtype or torch.float32, device=dev)
+    code = _float_code(out.dtype)
+    _need(code is not None and out.device == dev and out.shape == (m, n) and (n <= 1 or out.stride(1) == 1)
+          and (out_dtype is None or out.dtype == out_dtype), "out: rows [m][n] of fp32, bf16 or fp16 are needed")
+    _call("dllm_cuda_matmul_i8", dev, stream, m, n, k, ap, lda, _vector(a_scale, m, torch.float32, dev, "a_scale"), bp,
+          ldb, _vector(b_scale, n, torch.float32, dev, "b_scale"), float(softcap), out.data_ptr(),
+          out.stride(0) if m > 1 else max(out.stride(0), n), code,
+          None if status is None else _vector(status, 1, torch.int32, dev, "status"))
+    return out
+
+
+def lmhead_logits_i8(h, w, w_scale, *, norm_w=None, eps=1e-6, add_one=False, softcap=0.0, logits=None, status=None,
+                     workspace=None, stream=None):
+    """lmhead_logits with int8 output weights (dllm_cuda_lmhead_logits_i8): h fp32 [rows][hidden], w int8
+    [vocab][hidden] and w_scale fp32 [vocab] from quantize_rows_i8; returns fp32 logits [rows][vocab]."""
+    import torch
+
+    _need(h.is_cuda and h.dim() == 2 and h.dtype == torch.float32 and h.is_contiguous(),
+          "h: a contiguous fp32 [rows][hidden] CUDA tensor is needed")
+    dev = h.device
+    rows, hidden = h.shape
+    wp, vocab, hw, ldw = _codes(w, dev, "w")
+    _need(hidden == hw, f"h has {hidden} columns, w {hw}")
+    if logits is None:
+        logits = torch.empty(rows, vocab, dtype=torch.float32, device=dev)
+    if workspace is None:
+        workspace = torch.empty(load_library().dllm_cuda_lmhead_i8_workspace_bytes(rows, hidden), dtype=torch.uint8,
+                                device=dev)
+    _need(workspace.device == dev and workspace.is_contiguous(), f"workspace: contiguous, on {dev}")
+    _call("dllm_cuda_lmhead_logits_i8", dev, stream, rows, hidden, vocab, h.data_ptr(),
+          None if norm_w is None else _vector(norm_w, hidden, torch.float32, dev, "norm_w"), float(eps),
+          int(bool(add_one)), wp, ldw, _vector(w_scale, vocab, torch.float32, dev, "w_scale"), float(softcap),
+          _vector(logits, rows * vocab, torch.float32, dev, "logits"),
+          None if status is None else _vector(status, 1, torch.int32, dev, "status"), workspace.data_ptr(),
+          workspace.numel() * workspace.element_size())
+    return logits
+
+
+# ---- beam search ------------------------------------------------------------------------------
+
+def fill_beam_desc(logits, scores, k, *, mask=None, finished=None, eos=-1, lengths=None, length_penalty=0.0, out=None,
+                   out_finished=None, out_lengths=None, status=None, workspace=None):
+    """Builds a dllm_beam_desc from CUDA tensors; returns (desc, (score, parent, token), workspace)."""
+    import torch
+
+    code = _float_code(logits.dtype)
+    _need(logits.is_cuda and logits.dim() == 2 and code is not None,
+          "logits: a 2-D fp32, bf16 or fp16 CUDA tensor is needed")
+    dev = logits.device
+    _need(scores.dim() == 2, "scores: [batch][beams] is needed")
+    batch, beams = scores.shape
+    rows, vocab = logits.shape
+    _need(rows == batch * beams, f"logits have {rows} rows, scores {batch} x {beams}")
+    _need(vocab <= 1 or logits.stride(1) == 1, "logits: contiguous rows are needed")
+    k = int(k)
+    d = BeamDesc()
+    d.batch, d.beams, d.vocab, d.k, d.dtype = batch, beams, vocab, k, code
+    d.row_stride = logits.stride(0) if rows > 1 else max(logits.stride(0), vocab)
+    d.logits = logits.data_ptr()
+    d.scores = _vector(scores, rows, torch.float32, dev, "scores")
+    if mask is not None:
+        _need(mask.dtype in (torch.int32, torch.uint32) and mask.device == dev and mask.dim() == 2
+              and mask.shape[0] == rows and mask.shape[1] >= (vocab + 31) // 32
+              and (mask.stride(1) == 1 or mask.shape[1] == 1), "mask: int32 words [rows][(vocab + 31) / 32] are needed")
+        d.mask, d.mask_stride = mask.data_ptr(), mask.stride(0) if rows > 1 else max(mask.stride(0), mask.shape[1])
+    if finished is not None:
+        _need(finished.dtype in (torch.uint8, torch.bool), "finished: uint8 or bool is needed")
+        d.finished = _vector(finished, rows, finished.dtype, dev, "finished")
+    d.eos = int(eos)
+    if lengths is not None:
+        d.lengths = _vector(lengths, rows, torch.int32, dev, "lengths")
+    d.length_penalty = float(length_penalty)
+    if out is None:
+        buf = torch.empty(3, batch, max(k, 0), dtype=torch.int32, device=dev)
+        out = (buf[0].view(torch.float32), buf[1], buf[2])
+    score, parent, token = out
+    d.out_score = _vector(score, batch * k, torch.float32, dev, "out score")
+    d.out_parent = _vector(parent, batch * k, torch.int32, dev, "out parent")
+    d.out_token = _vector(token, batch * k, torch.int32, dev, "out token")
+    if out_finished is not None:
+        _need(out_finished.dtype in (torch.uint8, torch.bool), "out_finished: uint8 or bool is needed")
+        d.out_finished = _vector(out_finished, batch * k, out_finished.dtype, dev, "out_finished")
+    if out_lengths is not None:
+        d.out_lengths = _vector(out_lengths, batch * k, torch.int32, dev, "out_lengths")
+    if status is not None:
+        d.status = _vector(status, rows, torch.int32, dev, "status")
+    if workspace is None:
+        workspace = torch.empty(load_library().dllm_cuda_beam_workspace_bytes(C.byref(d)), dtype=torch.uint8,
+                                device=dev)
+    _need(workspace.device == dev and workspace.is_contiguous(), f"workspace: contiguous, on {dev}")
+    d.workspace, d.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    return d, out, workspace
+
+
+def beam_select(logits, scores, k, *, stream=None, **kw):
+    """The k best continuations of each sequence's beams (dllm_cuda_beam_select): logits [batch * beams]
+    [vocab], scores fp32 [batch][beams].  Returns (score fp32, parent int32, token int32), each
+    [batch][k], best rank first; a slot that nothing fills has (-inf, -1, -1).  Options: `mask`
+    (packed allow-bits), `finished` and `eos` (ended beams), `lengths` and `length_penalty`, `out`
+    (the three outputs), `out_finished`, `out_lengths`, `status`, `workspace`."""
+    d, out, ws = fill_beam_desc(logits, scores, k, **kw)
+    _call("dllm_cuda_beam_select", logits.device, stream, C.byref(d))
+    return out
+
+
+def _runs(t):
+    """(row stride, segments, segment stride, run), the last three in bytes as the row stride, of a
+    state [rows][...] whose inner dimensions are runs of one length at one stride."""
+    esz = t.element_size()
+    run, segs, seg_stride = esz, 1, 0
+    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if size == 1:
+            continue
+        if segs == 1 and stride * esz == run:
+            run *= size
+        elif segs == 1:
+            segs, seg_stride = size, stride * esz
+        else:
+            _need(stride * esz == segs * seg_stride, "a state's rows have to be runs at one stride")
+            segs *= size
+    return (t.stride(0) * esz, segs, seg_stride, run)
+
+
+def beam_reorder(states, parents, *, stream=None):
+    """Moves states after their beams' parents, in place (dllm_cuda_beam_reorder): every tensor of
+    `states` [batch * beams][...] gets row (s, b) from row (s, parents[s][b]); parents int32
+    [batch][beams], -1 leaves the beam as it is.  A view, such as the used part of a cache, is moved
+    without what lies around it."""
+    import torch
+
+    _need(parents.is_cuda and parents.dim() == 2 and parents.dtype == torch.int32 and parents.is_contiguous(),
+          "parents: contiguous int32 [batch][beams] on the GPU is needed")
+    dev = parents.device
+    batch, beams = parents.shape
+    groups = {}
+    for t in states:
+        _need(t.device == dev and t.dim() >= 1 and t.shape[0] == batch * beams,
+              f"a state of {batch * beams} rows on {dev} is needed")
+        if t.numel():
+            groups.setdefault(_runs(t), []).append(t.data_ptr())
+    _need(len({p for ptrs in groups.values() for p in ptrs}) == sum(map(len, groups.values())), "a state is given twice")
+    for (row, segs, seg, run), ptrs in groups.items():
+        _call("dllm_cuda_beam_reorder", dev, stream, batch, beams, parents.data_ptr(), len(ptrs),
+              (C.c_void_p * len(ptrs))(*ptrs), row, segs, seg, run)

@@ -221,6 +221,203 @@ extern "C" dllm_status dllm_cuda_lmhead_logits(int rows, int hidden, int vocab, 
 }
 
 // ----------------------------------------------------------------------------------------
+// int8 LM head
+
+static dllm_status invalid(const char *msg) {
+    set_last_error_message(msg);
+    return DLLM_ERR_INVALID_ARG;
+}
+
+static bool float_dtype(int t) { return t == DLLM_DTYPE_F32 || t == DLLM_DTYPE_BF16 || t == DLLM_DTYPE_F16; }
+
+static size_t dtype_bytes(int t) { return t == DLLM_DTYPE_F32 ? 4 : 2; }
+
+// Rows of int8 codes: base and stride on 16 bytes (the product's tiles are copied by 16-byte units).
+static bool codes_aligned(const void *p, int64_t stride, int cols) {
+    return (uintptr_t)p % 16 == 0 && stride % 16 == 0 && stride >= cols;
+}
+
+// A call's scratch: the caller's, or the library's buffer of the (device, stream).  The library's
+// may be freed and grown by a later call, which a captured graph would not see, and growing it is
+// not allowed during a capture: refused there.
+static dllm_status scratch_for(void *given, size_t given_bytes, size_t need, cudaStream_t stream, void **out) {
+    if (given) {
+        if ((uintptr_t)given % 256 != 0) return invalid("workspace is not 256-byte aligned");
+        if (given_bytes < need) return invalid("workspace is too small");
+        *out = given;
+        return DLLM_OK;
+    }
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    const cudaError_t e = cudaStreamIsCapturing(stream, &cap);
+    if (e != cudaSuccess) {
+        set_error("cudaStreamIsCapturing", e);
+        return DLLM_ERR_CUDA;
+    }
+    if (cap != cudaStreamCaptureStatusNone) return invalid("a captured call needs a workspace of the caller");
+    *out = internal_workspace((void *)stream, need);
+    if (!*out) {
+        set_error("scratch", cudaErrorMemoryAllocation);
+        return DLLM_ERR_OOM;
+    }
+    return DLLM_OK;
+}
+
+extern "C" dllm_status dllm_cuda_quantize_rows_i8(int rows, int cols, const void *x, int64_t x_stride, int x_dtype,
+                                                  int norm, const float *norm_w, float eps, int add_one, int8_t *q,
+                                                  int64_t q_stride, float *scale, void *stream) {
+    if (rows < 0 || cols < 1) return invalid("rows < 0 or cols < 1");
+    if (!float_dtype(x_dtype)) return invalid("x is fp32, bf16 or fp16");
+    if (rows == 0) return DLLM_OK;
+    if (!x || !q || !scale) return invalid("x, q and scale are needed");
+    if (x_stride < cols) return invalid("x_stride < cols");
+    if ((uintptr_t)x % dtype_bytes(x_dtype) != 0) return invalid("x is not aligned to its type");
+    if (!codes_aligned(q, q_stride, cols)) return invalid("q: base and stride on 16 bytes, stride >= cols");
+    if (!norm && (norm_w || add_one)) return invalid("norm_w and add_one belong to norm");
+    if (norm && !(eps >= 0.0f)) return invalid("eps < 0");
+    const dllm_status st = launch_quantize_i8(rows, cols, x, x_stride, x_dtype, norm, norm_w, eps, add_one, q, q_stride,
+                                              scale, (cudaStream_t)stream);
+    if (st == DLLM_ERR_CUDA) set_error("int8 quantisation kernel launch", cudaGetLastError());
+    return st;
+}
+
+static dllm_status check_matmul_i8(int m, int n, int k, float softcap) {
+    if (m < 0 || n < 0 || k < 1) return invalid("m < 0, n < 0 or k < 1");
+    if (!(softcap >= 0.0f && softcap <= 3.4e38f)) return invalid("softcap is 0 or a positive number");
+    if (k > 131071) {  // 128 * 128 * k has to stay below 2^31
+        set_last_error_message("k > 131071: the 32-bit sums could overflow");
+        return DLLM_ERR_UNSUPPORTED;
+    }
+    return DLLM_OK;
+}
+
+static dllm_status run_matmul_i8(int m, int n, int k, const int8_t *a, int64_t lda, const float *sa, const int8_t *b,
+                                 int64_t ldb, const float *sb, float softcap, void *out, int64_t ldo, int out_dtype,
+                                 int32_t *status, cudaStream_t stream) {
+    const dllm_status st = launch_matmul_i8(m, n, k, a, lda, sa, b, ldb, sb, softcap, out, ldo, out_dtype, status,
+                                            stream);
+    if (st == DLLM_ERR_CUDA) set_error("int8 product kernel launch", cudaGetLastError());
+    return st;
+}
+
+extern "C" dllm_status dllm_cuda_matmul_i8(int m, int n, int k, const int8_t *a, int64_t a_stride,
+                                           const float *a_scale, const int8_t *b, int64_t b_stride,
+                                           const float *b_scale, float softcap, void *out, int64_t out_stride,
+                                           int out_dtype, int32_t *status, void *stream) {
+    const dllm_status ok = check_matmul_i8(m, n, k, softcap);
+    if (ok != DLLM_OK) return ok;
+    if (!float_dtype(out_dtype)) return invalid("out is fp32, bf16 or fp16");
+    if (m == 0 || n == 0) return DLLM_OK;
+    if (!a || !a_scale || !b || !b_scale || !out) return invalid("a, b, their scales and out are needed");
+    if (!codes_aligned(a, a_stride, k) || !codes_aligned(b, b_stride, k))
+        return invalid("a and b: base and stride on 16 bytes, stride >= k");
+    if (out_stride < n) return invalid("out_stride < n");
+    if ((uintptr_t)out % dtype_bytes(out_dtype) != 0) return invalid("out is not aligned to its type");
+    return run_matmul_i8(m, n, k, a, a_stride, a_scale, b, b_stride, b_scale, softcap, out, out_stride, out_dtype,
+                         status, (cudaStream_t)stream);
+}
+
+static int64_t code_stride(int cols) { return ((int64_t)cols + 15) / 16 * 16; }
+
+extern "C" size_t dllm_cuda_lmhead_i8_workspace_bytes(int rows, int hidden) {
+    if (rows < 1 || hidden < 1) return 0;
+    return ((size_t)rows * code_stride(hidden) + 255) / 256 * 256 + (size_t)rows * sizeof(float);
+}
+
+extern "C" dllm_status dllm_cuda_lmhead_logits_i8(int rows, int hidden, int vocab, const float *h, const float *norm_w,
+                                                  float eps, int add_one, const int8_t *w, int64_t w_stride,
+                                                  const float *w_scale, float softcap, float *logits, int32_t *status,
+                                                  void *workspace, size_t workspace_bytes, void *stream) {
+    const dllm_status ok = check_matmul_i8(rows, vocab, hidden, softcap);
+    if (ok != DLLM_OK) return ok;
+    if (vocab < 1) return invalid("vocab < 1");
+    if (rows == 0) return DLLM_OK;
+    if (!h || !w || !w_scale || !logits) return invalid("h, w, w_scale and logits are needed");
+    if (!codes_aligned(w, w_stride, hidden)) return invalid("w: base and stride on 16 bytes, stride >= hidden");
+    if (!(eps >= 0.0f)) return invalid("eps < 0");
+    void *ws = nullptr;
+    dllm_status st = scratch_for(workspace, workspace_bytes, dllm_cuda_lmhead_i8_workspace_bytes(rows, hidden),
+                                 (cudaStream_t)stream, &ws);
+    if (st != DLLM_OK) return st;
+    int8_t *q = (int8_t *)ws;
+    float *scale = (float *)((unsigned char *)ws + ((size_t)rows * code_stride(hidden) + 255) / 256 * 256);
+    st = dllm_cuda_quantize_rows_i8(rows, hidden, h, hidden, DLLM_DTYPE_F32, 1, norm_w, eps, add_one, q,
+                                    code_stride(hidden), scale, stream);
+    if (st != DLLM_OK) return st;
+    return run_matmul_i8(rows, vocab, hidden, q, code_stride(hidden), scale, w, w_stride, w_scale, softcap, logits,
+                         vocab, DLLM_DTYPE_F32, status, (cudaStream_t)stream);
+}
+
+// ----------------------------------------------------------------------------------------
+// beam search
+
+static dllm_status check_beam(const dllm_beam_desc *d) {
+    if (!d) return invalid("no descriptor");
+    if (d->batch < 0 || d->beams < 1 || d->vocab < 1 || d->k < 1) return invalid("a size is out of range");
+    if (!float_dtype(d->dtype)) return invalid("logits are fp32, bf16 or fp16");
+    if (d->beams > DLLM_BEAM_MAX || d->k > DLLM_BEAM_K_MAX) {
+        set_last_error_message("more than 128 beams or 256 continuations");
+        return DLLM_ERR_UNSUPPORTED;
+    }
+    if (d->row_stride < d->vocab) return invalid("row_stride < vocab");
+    if (d->mask && d->mask_stride < ((int64_t)d->vocab + 31) / 32) return invalid("mask_stride is too small");
+    if (!(d->length_penalty >= -3.4e38f && d->length_penalty <= 3.4e38f)) return invalid("length_penalty is not finite");
+    if ((d->length_penalty != 0.0f || d->out_lengths) && !d->lengths) return invalid("lengths are needed");
+    if ((d->finished || d->out_finished) && d->eos < 0) return invalid("eos < 0");
+    if (d->batch == 0) return DLLM_OK;
+    if (!d->logits || !d->scores || !d->out_score || !d->out_parent || !d->out_token)
+        return invalid("logits, scores and the three outputs are needed");
+    if ((uintptr_t)d->logits % dtype_bytes(d->dtype) != 0) return invalid("logits are not aligned to their type");
+    return DLLM_OK;
+}
+
+extern "C" size_t dllm_cuda_beam_workspace_bytes(const dllm_beam_desc *d) {
+    if (!d || d->batch < 1 || d->beams < 1 || d->vocab < 1 || d->k < 1 || d->beams > DLLM_BEAM_MAX ||
+        d->k > DLLM_BEAM_K_MAX || !float_dtype(d->dtype))
+        return 0;
+    return beam_ws_bytes(d);
+}
+
+extern "C" dllm_status dllm_cuda_beam_select(const dllm_beam_desc *d, void *stream) {
+    dllm_status st = check_beam(d);
+    if (st != DLLM_OK) return st;
+    if (d->batch == 0) return DLLM_OK;
+    void *ws = nullptr;
+    st = scratch_for(d->workspace, d->workspace_bytes, beam_ws_bytes(d), (cudaStream_t)stream, &ws);
+    if (st != DLLM_OK) return st;
+    st = launch_beam_select(d, ws, (cudaStream_t)stream);
+    if (st == DLLM_ERR_CUDA) set_error("beam selection kernel launch", cudaGetLastError());
+    else if (st != DLLM_OK) set_last_error_message("too many rows for one call");
+    return st;
+}
+
+extern "C" dllm_status dllm_cuda_beam_reorder(int batch, int beams, const int32_t *parent, int ntensors,
+                                              void *const *tensors, int64_t row_stride, int segs, int64_t seg_stride,
+                                              int64_t run_bytes, void *stream) {
+    if (batch < 0 || beams < 1 || ntensors < 0 || segs < 0 || run_bytes < 0) return invalid("a size is out of range");
+    if (beams > DLLM_BEAM_MAX) {
+        set_last_error_message("more than 128 beams");
+        return DLLM_ERR_UNSUPPORTED;
+    }
+    if (batch == 0 || ntensors == 0 || segs == 0 || run_bytes == 0) return DLLM_OK;
+    if (!parent || !tensors) return invalid("parent and tensors are needed");
+    // no two runs of a tensor may overlap: rows around segments, or segments around rows
+    const __int128 rows = (__int128)batch * beams, run = run_bytes, rs = row_stride, ss = seg_stride;
+    bool fits = (rows == 1 || rs >= run) && (segs == 1 || ss >= run);
+    if (rows > 1 && segs > 1) fits = fits && (rs >= (segs - 1) * ss + run || ss >= (rows - 1) * rs + run);
+    if (!fits) return invalid("runs of a state overlap");
+    for (int i = 0; i < ntensors; i++) {
+        if (!tensors[i]) return invalid("a state is NULL");
+        for (int j = 0; j < i; j++)
+            if (tensors[i] == tensors[j]) return invalid("a state is given twice");
+    }
+    const dllm_status st = launch_beam_reorder(batch, beams, parent, ntensors, tensors, row_stride, segs, seg_stride,
+                                               run_bytes, (cudaStream_t)stream);
+    if (st == DLLM_ERR_CUDA) set_error("beam reorder kernel launch", cudaGetLastError());
+    else if (st != DLLM_OK) set_last_error_message("state too large for one call");
+    return st;
+}
+
+// ----------------------------------------------------------------------------------------
 // vocabulary-sharded sampling (no counterpart in the reference, whose sampler sees whole rows)
 
 extern "C" dllm_status dllm_cuda_shard_candidates(const dllm_batch_desc *d, int64_t vocab_offset, int64_t vocab_total,

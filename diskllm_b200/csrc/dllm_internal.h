@@ -119,6 +119,16 @@ int lmh_max_rows(int hidden);
 dllm_status launch_lmhead(int rows, int hidden, int vocab, const float *h, const float *norm_w, float eps, int add_one,
                           const void *w, int w_dtype, float softcap, float *logits, float *scratch,
                           cudaStream_t stream);
+dllm_status launch_quantize_i8(int rows, int cols, const void *x, int64_t x_stride, int x_dtype, int norm,
+                               const float *norm_w, float eps, int add_one, int8_t *q, int64_t q_stride, float *scale,
+                               cudaStream_t stream);
+dllm_status launch_matmul_i8(int m, int n, int k, const int8_t *a, int64_t lda, const float *sa, const int8_t *b,
+                             int64_t ldb, const float *sb, float softcap, void *out, int64_t ldo, int out_dtype,
+                             int32_t *status, cudaStream_t stream);
+size_t beam_ws_bytes(const dllm_beam_desc *d);
+dllm_status launch_beam_select(const dllm_beam_desc *d, void *ws, cudaStream_t stream);
+dllm_status launch_beam_reorder(int batch, int beams, const int32_t *parent, int ntensors, void *const *tensors,
+                                int64_t row_stride, int segs, int64_t seg_stride, int64_t run, cudaStream_t stream);
 // Peer exchange of vocabulary-sharded candidates (see dllm_cuda_peer_exchange_create).
 struct PeerArgs {
     void *const *peers;         // device array [world] of every rank's exchange buffer, mapped here

@@ -6,6 +6,9 @@ kernels' time and no host round trip.
 
 The logits of step i are row i % R of a device ring (a real model writes them in place each step;
 here they are given), the uniform of step i is uniforms[i] (one U[0,1) per step).
+
+BeamLoop is the same for beam search: LM head with int8 weights, selection over beams and
+vocabulary, states moved after their parents.
 """
 from __future__ import annotations
 
@@ -67,6 +70,96 @@ class DecodeLoop:
         launch configuration outside the capture)."""
         self._reset()
         self._step(0)
+        torch.cuda.synchronize(self.dev)
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph):
+            self._reset()
+            for i in range(self.steps):
+                self._step(i)
+        return self
+
+    def replay(self) -> torch.Tensor:
+        if self.graph is None:
+            self.capture()
+        self.graph.replay()
+        return self.tokens
+
+
+class BeamLoop:
+    """Beam search over `batch` sequences of `beams` beams.  A step takes the hidden states of every
+    beam (entry i % R of hidden_ring [R][batch * beams][hidden], fp32), forms their logits with int8
+    output weights (wq, w_scale from capi.quantize_rows_i8), selects the best `beams` continuations
+    of each sequence, moves `states` (tensors [batch * beams][...], such as caches) and the token
+    histories after their parents, and appends the new tokens.  The first step starts from one live
+    beam per sequence.  A beam that has produced `eos` stays as it is.
+
+    After a run: tokens [batch][beams][steps] int32 (best beam first; after an end the token is eos,
+    in slots that nothing filled -1), scores [batch][beams], lengths and finished."""
+
+    def __init__(self, hidden_ring: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, batch: int, beams: int,
+                 steps: int, *, eos: int, length_penalty: float = 0.0, norm_w: torch.Tensor | None = None,
+                 eps: float = 1e-6, add_one: bool = False, softcap: float = 0.0, states=(),
+                 mask_ring: torch.Tensor | None = None):
+        assert hidden_ring.is_cuda and hidden_ring.dim() == 3 and hidden_ring.shape[1] == batch * beams
+        self.dev = hidden_ring.device
+        self.ring, self.wq, self.w_scale = hidden_ring, wq, w_scale
+        self.batch, self.beams, self.steps = batch, beams, steps
+        self.eos, self.length_penalty = eos, length_penalty
+        self.head = dict(norm_w=norm_w, eps=eps, add_one=add_one, softcap=softcap)
+        self.states = list(states)
+        self.mask_ring = mask_ring
+        rows = batch * beams
+
+        def buf(*shape, dtype=torch.int32):
+            return torch.zeros(*shape, dtype=dtype, device=self.dev)
+
+        self.scores, self.lengths = buf(batch, beams, dtype=torch.float32), buf(batch, beams)
+        self.finished = buf(batch, beams, dtype=torch.uint8)
+        self.parents, self.new = buf(batch, beams), buf(batch, beams)
+        self.hist = buf(rows, steps)
+        self.first = torch.full((batch, beams), float("-inf"), device=self.dev)
+        self.first[:, 0] = 0.0
+        # buffers given to every call, so that nothing is allocated inside a capture
+        self.logits = buf(rows, wq.shape[0], dtype=torch.float32)
+        self.head_ws = buf(max(1, capi.load_library().dllm_cuda_lmhead_i8_workspace_bytes(rows, wq.shape[1])),
+                           dtype=torch.uint8)
+        _, _, self.beam_ws = capi.fill_beam_desc(self.logits, self.scores, beams, eos=eos)
+        self.graph = None
+
+    @property
+    def tokens(self) -> torch.Tensor:
+        return self.hist.view(self.batch, self.beams, self.steps)
+
+    def _reset(self):
+        self.scores.copy_(self.first)
+        self.lengths.zero_()
+        self.finished.zero_()
+
+    def _step(self, i: int):
+        r = i % self.ring.shape[0]
+        capi.lmhead_logits_i8(self.ring[r], self.wq, self.w_scale, logits=self.logits, workspace=self.head_ws, **self.head)
+        capi.beam_select(self.logits, self.scores, self.beams, finished=self.finished, eos=self.eos,
+                         mask=None if self.mask_ring is None else self.mask_ring[r],
+                         lengths=self.lengths, length_penalty=self.length_penalty,
+                         out=(self.scores, self.parents, self.new), out_finished=self.finished,
+                         out_lengths=self.lengths, workspace=self.beam_ws)
+        capi.beam_reorder([self.hist[:, :i], *self.states], self.parents)
+        self.hist[:, i].copy_(self.new.view(-1))
+
+    def run_eager(self) -> torch.Tensor:
+        """Every step launched from the host."""
+        self._reset()
+        for i in range(self.steps):
+            self._step(i)
+        return self.tokens
+
+    def capture(self):
+        """Records reset + all steps as one CUDA graph.  Nothing runs on the states before it: the
+        library is warmed up by one product and one selection on this loop's own buffers."""
+        capi.lmhead_logits_i8(self.ring[0], self.wq, self.w_scale, logits=self.logits, workspace=self.head_ws, **self.head)
+        self._reset()
+        capi.beam_select(self.logits, self.scores, self.beams, out=(self.scores, self.parents, self.new),
+                         workspace=self.beam_ws)
         torch.cuda.synchronize(self.dev)
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):

@@ -44,7 +44,7 @@ typedef enum {
 enum {
     DLLM_DTYPE_F32 = 0,
     DLLM_DTYPE_BF16 = 1,
-    DLLM_DTYPE_F16 = 2,   /* output weights of dllm_cuda_lmhead_logits only */
+    DLLM_DTYPE_F16 = 2,   /* dllm_cuda_lmhead_logits's output weights, the int8 and beam calls */
 };
 
 /* mode flags */
@@ -255,6 +255,99 @@ DLLM_API dllm_status dllm_cuda_merge_sample_peer(int rows, int world, int k, con
 DLLM_API dllm_status dllm_cuda_lmhead_logits(int rows, int hidden, int vocab, const float *h, const float *norm_w,
                                              float eps, int add_one, const void *w, int w_dtype, float softcap,
                                              float *logits, void *stream);
+
+/* The LM-head tail with 8-bit integer weights (no counterpart in the reference).  Codes are
+ * symmetric, from -127 to 127, with one fp32 scale for each row; rows of codes start on multiples
+ * of 16 bytes (base and stride), so a row may be followed by padding, which is not read as data.
+ *
+ * dllm_cuda_quantize_rows_i8: `rows` rows of `cols` values (fp32 / bf16 / fp16, x_stride elements
+ *   apart) to codes q [rows][q_stride] and scales [rows].  Without norm y = x; with norm
+ *   y = x * g / sqrt(mean(x^2) + eps), g = norm_w, norm_w + 1 (add_one) or 1 (norm_w NULL).
+ *   scale = (float)(max|y| / 127) and q = y / scale rounded to the nearest integer, ties to even,
+ *   both decided in 64 bits.  A row whose scale would lie below the smallest normal float has
+ *   scale 0 and codes 0; a row with an infinity or a NaN has scale NaN and codes 0.  Quantises
+ *   output weights (rows = vocabulary) once, and activations (rows = tokens) each step.
+ *   Padding behind a row is left as it was.
+ * dllm_cuda_matmul_i8: out[i][j] = a_scale[i] * b_scale[j] * sum over k of a[i][k] * b[j][k], for m
+ *   rows of a (tokens) and n rows of b (channels): the sum exact in 32-bit integers
+ *   (k <= 131071), then two fp32 products, the softcap cap * tanhf(out / cap) when softcap > 0,
+ *   and one rounding to out_dtype (fp32 / bf16 / fp16).  Codes may be -128 too.
+ *   status (optional, one device word): DLLM_ROW_ERR_TIMEOUT is ORed in if a bounded wait expired.
+ * dllm_cuda_lmhead_logits_i8: dllm_cuda_lmhead_logits with int8 output weights w [vocab][w_stride]
+ *   and their scales: the final RMSNorm and the codes of h [rows][hidden] in one kernel, then the
+ *   product and the softcap, writing fp32 logits [rows][vocab].  `workspace` holds the codes
+ *   (dllm_cuda_lmhead_i8_workspace_bytes, 256-byte aligned); NULL: the library's buffer of the
+ *   (device, stream), which is refused while the stream is being captured. */
+DLLM_API dllm_status dllm_cuda_quantize_rows_i8(int rows, int cols, const void *x, int64_t x_stride, int x_dtype,
+                                                int norm, const float *norm_w, float eps, int add_one, int8_t *q,
+                                                int64_t q_stride, float *scale, void *stream);
+DLLM_API dllm_status dllm_cuda_matmul_i8(int m, int n, int k, const int8_t *a, int64_t a_stride, const float *a_scale,
+                                         const int8_t *b, int64_t b_stride, const float *b_scale, float softcap,
+                                         void *out, int64_t out_stride, int out_dtype, int32_t *status, void *stream);
+DLLM_API size_t dllm_cuda_lmhead_i8_workspace_bytes(int rows, int hidden);
+DLLM_API dllm_status dllm_cuda_lmhead_logits_i8(int rows, int hidden, int vocab, const float *h, const float *norm_w,
+                                                float eps, int add_one, const int8_t *w, int64_t w_stride,
+                                                const float *w_scale, float softcap, float *logits, int32_t *status,
+                                                void *workspace, size_t workspace_bytes, void *stream);
+
+/* One step of beam search (no counterpart in the reference, which draws one token per row).
+ *
+ * dllm_cuda_beam_select: for each of `batch` sequences, the k best continuations of its `beams`
+ * beams.  With lp(b, i) = x_bi - log(sum over allowed j of exp(x_bj)) over beam b's logits row,
+ * a continuation (b, i) has the score cum = scores[b] + lp(b, i) and the rank cum / L^alpha, where
+ * L = lengths[b] + 1 is its length in tokens (alpha = length_penalty; without lengths or with
+ * alpha = 0 the rank is the score).  Order: rank descending, then beam, then logit descending,
+ * then id ascending; sums and ranks are held in 64 bits.
+ *   - A cleared mask bit leaves id i out, whatever its logit.  Continuations of probability 0
+ *     (logit -inf, score -inf) are never chosen: slots that nothing fills get score -inf,
+ *     parent -1, token -1.
+ *   - An ended beam (finished[b] != 0) has one continuation, the token `eos` with its own score
+ *     and L = max(lengths[b], 1); its logits are not read.
+ *   - A row with an unmasked NaN or +inf, or a score of NaN or +inf, offers nothing; its status
+ *     word gets DLLM_ROW_ERR_NONFINITE.
+ * beams <= DLLM_BEAM_MAX, k <= DLLM_BEAM_K_MAX.  Outputs may be the arrays of the inputs of the
+ * same shape (k = beams).
+ *
+ * dllm_cuda_beam_reorder: state[s][b] = state[s][parent[s][b]] for each of `ntensors` tensors, in
+ * place (parent: device [batch][beams], values outside 0 .. beams - 1 leave the beam as it is).
+ * `tensors` is a HOST array of device pointers, no two equal; each tensor holds batch x beams rows
+ * row_stride bytes apart, a row being `segs` runs of run_bytes bytes, seg_stride bytes apart.
+ * Bytes between runs are not touched.  Beams that keep their own state are neither read nor
+ * written. */
+#define DLLM_BEAM_MAX   128
+#define DLLM_BEAM_K_MAX 256
+
+typedef struct {
+    int batch, beams, vocab, k;
+    int64_t row_stride;       /* elements between consecutive rows (>= vocab) */
+    int dtype;                /* DLLM_DTYPE_F32 / BF16 / F16 */
+    const void *logits;       /* [batch * beams][row_stride] */
+    const uint32_t *mask;     /* allow-mask of each row or NULL, as in dllm_batch_desc */
+    int64_t mask_stride;      /* words between rows */
+    const float *scores;      /* [batch][beams] sums of log-probabilities so far */
+    const uint8_t *finished;  /* [batch][beams] ended beams, or NULL */
+    int eos;                  /* end token (>= 0 when finished or out_finished is given) */
+    const int32_t *lengths;   /* [batch][beams] tokens so far, or NULL */
+    float length_penalty;     /* alpha; finite, needs lengths when it is not 0 */
+
+    float *out_score;         /* [batch][k] scores (not ranks), best rank first */
+    int32_t *out_parent;      /* [batch][k] beam that each continues */
+    int32_t *out_token;       /* [batch][k] id that it adds */
+    uint8_t *out_finished;    /* optional [batch][k]: ended before, or by this token */
+    int32_t *out_lengths;     /* optional [batch][k]: tokens including this one; needs lengths */
+    int32_t *status;          /* optional [batch][beams] out: 0 or DLLM_ROW_ERR_NONFINITE */
+
+    void *workspace;          /* device scratch of dllm_cuda_beam_workspace_bytes() bytes, 256-byte
+                                 aligned; NULL: the library's buffer of the (device, stream),
+                                 refused while the stream is being captured */
+    size_t workspace_bytes;
+} dllm_beam_desc;
+
+DLLM_API size_t dllm_cuda_beam_workspace_bytes(const dllm_beam_desc *desc);
+DLLM_API dllm_status dllm_cuda_beam_select(const dllm_beam_desc *desc, void *stream);
+DLLM_API dllm_status dllm_cuda_beam_reorder(int batch, int beams, const int32_t *parent, int ntensors,
+                                            void *const *tensors, int64_t row_stride, int segs, int64_t seg_stride,
+                                            int64_t run_bytes, void *stream);
 
 /* Decode-loop glue (no counterpart in the reference, whose caller appends to its seen-token
  * array on the host): appends token[0] (device) to one sequence's device history
