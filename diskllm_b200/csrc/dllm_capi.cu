@@ -267,6 +267,10 @@ extern "C" dllm_status dllm_cuda_quantize_rows_i8(int rows, int cols, const void
                                                   int64_t q_stride, float *scale, void *stream) {
     if (rows < 0 || cols < 1) return invalid("rows < 0 or cols < 1");
     if (!float_dtype(x_dtype)) return invalid("x is fp32, bf16 or fp16");
+    if (cols > (1 << 30)) {
+        set_last_error_message("more than 2^30 columns");
+        return DLLM_ERR_UNSUPPORTED;
+    }
     if (rows == 0) return DLLM_OK;
     if (!x || !q || !scale) return invalid("x, q and scale are needed");
     if (x_stride < cols) return invalid("x_stride < cols");
@@ -283,6 +287,10 @@ extern "C" dllm_status dllm_cuda_quantize_rows_i8(int rows, int cols, const void
 static dllm_status check_matmul_i8(int m, int n, int k, float softcap) {
     if (m < 0 || n < 0 || k < 1) return invalid("m < 0, n < 0 or k < 1");
     if (!(softcap >= 0.0f && softcap <= 3.4e38f)) return invalid("softcap is 0 or a positive number");
+    if (m > (1 << 30) || n > (1 << 30)) {
+        set_last_error_message("more than 2^30 rows of codes");
+        return DLLM_ERR_UNSUPPORTED;
+    }
     if (k > 131071) {  // 128 * 128 * k has to stay below 2^31
         set_last_error_message("k > 131071: the 32-bit sums could overflow");
         return DLLM_ERR_UNSUPPORTED;
