@@ -21,7 +21,8 @@ namespace {
 constexpr int BS_NT = 256;
 constexpr int BS_WARPS = BS_NT / 32;
 constexpr int BS_U = 4;             // 16-byte vectors per thread and tile
-constexpr int BS_CAP = 4096;        // candidate buffer (entries of 8 bytes); a power of two
+constexpr int BS_WCAP = 512;        // candidates that a warp holds: at least k (256) and one vector of each lane
+constexpr int BS_CAP = BS_WARPS * BS_WCAP;
 constexpr uint32_t KEY_NINF = 0x007fffffu;  // order key of -inf
 
 // One chunk's maximum and exponential sum relative to it.
@@ -45,6 +46,27 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Maximum that keeps subnormal values (the unit is built to flush them) and passes over NaN.
+__device__ __forceinline__ float max_keep(float a, float b) {
+    float y;
+    asm("max.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+// Two fp32 additions or products in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 y;
+    asm("{\n.reg .b64 a, b, y;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.ftz.f32x2 y, a, b;\nmov.b64 {%0, %1}, y;\n}"
+        : "=f"(y.x), "=f"(y.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return y;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 y;
+    asm("{\n.reg .b64 a, b, y;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.ftz.f32x2 y, a, b;\nmov.b64 {%0, %1}, y;\n}"
+        : "=f"(y.x), "=f"(y.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return y;
+}
 
 // A candidate: (order key << 32) | ~id, so that a larger composite is (logit desc, id asc).
 __device__ __forceinline__ uint64_t composite(uint32_t key, int id) { return (uint64_t)key << 32 | (uint32_t)~id; }
@@ -55,13 +77,12 @@ __device__ __forceinline__ bool beam_live(const dllm_beam_desc &d, int64_t row) 
     return fabsf(d.scores[row]) <= FLT_MAX;
 }
 
-// Sorts buf[0, n2) descending (n2 a power of two; entries past n are set to 0 first).
-__device__ void sort_desc(uint64_t *buf, int n, int n2) {
-    for (int i = n + threadIdx.x; i < n2; i += BS_NT) buf[i] = 0;
-    __syncthreads();
+// Sorts buf[0, n2) descending (n2 a power of two) by `nt` threads, of which this is number `t`.
+template <class Sync>
+__device__ __forceinline__ void sort_desc(uint64_t *buf, int n2, int t, int nt, Sync sync) {
     for (int size = 2; size <= n2; size <<= 1)
         for (int stride = size >> 1; stride; stride >>= 1) {
-            for (int i = threadIdx.x; i < n2 / 2; i += BS_NT) {
+            for (int i = t; i < n2 / 2; i += nt) {
                 const int lo = 2 * i - (i & (stride - 1)), hi = lo + stride;
                 const uint64_t a = buf[lo], b = buf[hi];
                 if ((a < b) == ((lo & size) == 0)) {
@@ -69,219 +90,297 @@ __device__ void sort_desc(uint64_t *buf, int n, int n2) {
                     buf[hi] = a;
                 }
             }
-            __syncthreads();
+            sync();
         }
 }
 
-__device__ __forceinline__ int pow2_at_least(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
-
 // The j-th largest of a warp's 32 keys (j from 1), in every lane.
 __device__ __forceinline__ uint32_t warp_jth(uint32_t key, int j) {
-    uint32_t mx = 0;
-    for (int i = 0; i < j; i++) {
-        mx = __reduce_max_sync(0xffffffffu, key);
+    uint32_t mx = __reduce_max_sync(0xffffffffu, key);
+    for (int i = 1; i < j; i++) {
         const uint32_t holders = __ballot_sync(0xffffffffu, key == mx);
         if ((threadIdx.x & 31) == __ffs(holders) - 1) key = 0;
+        mx = __reduce_max_sync(0xffffffffu, key);
     }
     return mx;
 }
 
+// How 16 bytes hold logits.
 template <int DT>
 struct Vec {
-    static constexpr int N = DT == DLLM_DTYPE_F32 ? 4 : 8;  // elements of 16 bytes
+    static constexpr int N = DT == DLLM_DTYPE_F32 ? 4 : 8;  // elements
+    static constexpr int ESZ = DT == DLLM_DTYPE_F32 ? 4 : 2;
+    static constexpr uint32_t NINF = DT == DLLM_DTYPE_F32 ? 0xff800000u : DT == DLLM_DTYPE_BF16 ? 0xff80ff80u : 0xfc00fc00u;
 };
 
+__device__ __forceinline__ uint32_t word_of(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// the two elements of word i of a 16-bit vector, or elements 2 i and 2 i + 1 of an fp32 one
 template <int DT>
-__device__ __forceinline__ void unpack(const uint4 &raw, float *f) {
-    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
-    if (DT == DLLM_DTYPE_F32) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) f[i] = __uint_as_float(u[i]);
+__device__ __forceinline__ float2 pair_of(const uint4 &v, int i) {
+    if (DT == DLLM_DTYPE_F32) return make_float2(__uint_as_float(word_of(v, 2 * i)), __uint_as_float(word_of(v, 2 * i + 1)));
+    const uint32_t u = word_of(v, i);
+    if (DT == DLLM_DTYPE_BF16) return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    return make_float2(__half2float(__ushort_as_half((unsigned short)(u & 0xffffu))),
+                       __half2float(__ushort_as_half((unsigned short)(u >> 16))));
+}
+
+// largest element of a vector
+template <int DT>
+__device__ __forceinline__ float vec_max(const uint4 &v) {
+    if (DT == DLLM_DTYPE_F32)
+        return max_keep(max_keep(__uint_as_float(v.x), __uint_as_float(v.y)),
+                        max_keep(__uint_as_float(v.z), __uint_as_float(v.w)));
+    uint32_t a, b, c;
+    if (DT == DLLM_DTYPE_BF16) {
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(v.x), "r"(v.y));
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(v.z), "r"(v.w));
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
     } else {
+        asm("max.f16x2 %0, %1, %2;" : "=r"(a) : "r"(v.x), "r"(v.y));
+        asm("max.f16x2 %0, %1, %2;" : "=r"(b) : "r"(v.z), "r"(v.w));
+        asm("max.f16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+    }
+    const float2 p = pair_of<DT>(make_uint4(c, 0, 0, 0), 0);
+    return max_keep(p.x, p.y);
+}
+
+template <int DT>
+__device__ __forceinline__ uint4 ninf_vector() {
+    return make_uint4(Vec<DT>::NINF, Vec<DT>::NINF, Vec<DT>::NINF, Vec<DT>::NINF);
+}
+
+// The vector of elements i0 .. of a row, of which some lie outside it: those and masked ones are -inf.
+template <int DT>
+__device__ __noinline__ uint4 edge_vector(const unsigned char *row, const uint32_t *mask, int i0, int V) {
+    constexpr int VEC = Vec<DT>::N;
+    uint32_t x[4] = {Vec<DT>::NINF, Vec<DT>::NINF, Vec<DT>::NINF, Vec<DT>::NINF};
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (DT == DLLM_DTYPE_BF16) {
-                f[2 * i] = __uint_as_float(u[i] << 16);
-                f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-            } else {
-                f[2 * i] = __half2float(__ushort_as_half((unsigned short)(u[i] & 0xffffu)));
-                f[2 * i + 1] = __half2float(__ushort_as_half((unsigned short)(u[i] >> 16)));
-            }
+    for (int e = 0; e < VEC; e++) {
+        if (i0 + e < 0 || e >= V - i0) continue;
+        const int i = i0 + e;
+        if (mask && !(mask[i >> 5] >> (i & 31) & 1)) continue;
+        if (DT == DLLM_DTYPE_F32) x[e % 4] = ((const uint32_t *)row)[i];
+        else {
+            const uint32_t u = ((const unsigned short *)row)[i];
+            x[e / 2] = e & 1 ? (x[e / 2] & 0xffffu) | u << 16 : (x[e / 2] & 0xffff0000u) | u;
         }
     }
+    return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
 // Grid rows x chunks.  A chunk is a range of the row's 16-byte vectors, counted from the row's
 // first byte rounded down to 16 (so any row start is served; the first and the last vector are
-// read by element).  Per tile a thread keeps its elements in registers, updates its running
-// maximum and sum, and appends those at or above the threshold to the candidate buffer.
+// read by element).  Per tile a thread updates its running maximum and exponential sum, and a warp
+// that holds an element at or above the threshold appends such elements to its own buffer; no
+// barrier is needed between tiles.
 //
-// Threshold: after the first tile, with k <= 8 j, the smallest over the warps of the j-th largest
-// thread maximum has at least k entries at or above it, all of the first tile, so with smaller
-// ids than any later entry; later ones have to be strictly larger.  When the buffer could
-// overflow it is sorted and cut to k, which raises the threshold the same way.
+// Threshold: with k <= 8 j, the smallest over the 8 warps of the j-th largest of the lanes' running
+// maxima has at least k different elements at or above it.  Each warp publishes its j-th largest
+// when it meets a candidate; an old one is lower, so no order between the warps is needed.  A warp
+// whose buffer could overflow sorts it and keeps its k best: their last key is a threshold for
+// all, and what the warp meets later, with larger ids, has to be strictly above it.
 template <int DT, bool MASK>
-__global__ void __launch_bounds__(BS_NT) beam_chunk_kernel(dllm_beam_desc d, int chunks, ChunkSum *sums,
-                                                           uint64_t *cands) {
-    constexpr int VEC = Vec<DT>::N, E = BS_U * VEC;
+__global__ void __launch_bounds__(BS_NT, 4) beam_chunk_kernel(dllm_beam_desc d, int chunks, ChunkSum *sums,
+                                                              uint64_t *cands) {
+    constexpr int VEC = Vec<DT>::N;
     constexpr float LOG2E = 1.44269504088896340736f;
     __shared__ uint64_t buf[BS_CAP];
-    __shared__ int count;
-    __shared__ uint32_t wkey[BS_WARPS];
+    __shared__ uint64_t few[BS_NT];
+    __shared__ volatile uint32_t wkey[BS_WARPS];
+    __shared__ uint32_t floor_key;
     __shared__ float wm[BS_WARPS];
     __shared__ double ws[BS_WARPS];
+    __shared__ int wcount[BS_WARPS];
+    asm volatile("griddepcontrol.launch_dependents;");
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const int64_t row = blockIdx.x / chunks;
     const int part_no = blockIdx.x % chunks;
     if (!beam_live(d, row)) return;
-    const int V = d.vocab, k = d.k;
-    const size_t esz = DT == DLLM_DTYPE_F32 ? 4 : 2;
-    const unsigned char *first = (const unsigned char *)d.logits + (size_t)row * d.row_stride * esz;
-    const int shift = (int)((uintptr_t)first % 16 / esz);  // elements before the row in its first vector
-    const uint4 *vecs = (const uint4 *)(first - shift * esz);
+    const int V = d.vocab, k = d.k, jth = (k + BS_WARPS - 1) / BS_WARPS;
+    const unsigned char *first = (const unsigned char *)d.logits + (size_t)row * d.row_stride * Vec<DT>::ESZ;
+    const int shift = (int)((uintptr_t)first % 16 / Vec<DT>::ESZ);  // elements before the row in its first vector
+    const uint4 *vecs = (const uint4 *)(first - shift * Vec<DT>::ESZ);
     const uint32_t *mrow = MASK ? d.mask + row * d.mask_stride : nullptr;
-    const int64_t nvec = ((int64_t)V + shift + VEC - 1) / VEC;
-    const int64_t per = (nvec + chunks - 1) / chunks;
-    const int64_t v0 = per * part_no, v1 = v0 + per < nvec ? v0 + per : nvec;
+    const int nvec = (int)(((int64_t)V + shift + VEC - 1) / VEC), per = (nvec + chunks - 1) / chunks;
+    const int v0 = per * part_no, v1 = min(v0 + per, nvec);
 
-    if (tid == 0) count = 0;
+    if (tid < BS_WARPS) wkey[tid] = 0;
+    if (tid == 0) floor_key = 0;
     __syncthreads();
 
-    // vector j as floats; masked elements and those outside the row are -inf
-    auto load = [&](int64_t j, float *f) {
-        if (j >= v1) {
+    // Vector j; masked elements and those outside the row are -inf.  A vector that is wholly masked
+    // is not read.
+    auto load = [&](int j) {
+        if (j >= v1) return ninf_vector<DT>();
+        const int i0 = j * VEC - shift;
+        if (i0 < 0 || i0 > V - VEC) return edge_vector<DT>(first, mrow, i0, V);
+        if (!MASK) return __ldg(vecs + j);
+        const int w = i0 >> 5, o = i0 & 31;
+        const uint32_t lo = __ldg(mrow + w), hi = o + VEC > 32 ? __ldg(mrow + w + 1) : 0;
+        const uint32_t bits = __funnelshift_r(lo, hi, o) & ((1u << VEC) - 1);
+        uint4 v = ninf_vector<DT>();
+        if (bits) v = __ldg(vecs + j);
+        uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int e = 0; e < VEC; e++) f[e] = -INFINITY;
-            return;
-        }
-        const int64_t i0 = j * VEC - shift;
-        if (i0 >= 0 && i0 + VEC <= V) {
-            unpack<DT>(__ldg(vecs + j), f);
-            if (MASK) {
-                const int w = (int)(i0 >> 5), o = (int)(i0 & 31);
-                const uint32_t lo = mrow[w], hi = o + VEC > 32 ? mrow[w + 1] : 0;
-                const uint32_t bits = __funnelshift_r(lo, hi, o);
-#pragma unroll
-                for (int e = 0; e < VEC; e++)
-                    if (!(bits >> e & 1)) f[e] = -INFINITY;
+        for (int i = 0; i < 4; i++) {
+            uint32_t keep;
+            if (DT == DLLM_DTYPE_F32) keep = 0u - (bits >> i & 1);
+            else {
+                const uint32_t two = bits >> (2 * i);
+                keep = ((two | two << 15) & 0x10001u) * 0xffffu;
             }
-        } else {
-#pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                const int64_t i = i0 + e;
-                float x = -INFINITY;
-                if (i >= 0 && i < V && (!MASK || (mrow[i >> 5] >> (i & 31) & 1))) {
-                    if (DT == DLLM_DTYPE_F32) x = ((const float *)first)[i];
-                    else {
-                        const unsigned short u = ((const unsigned short *)first)[i];
-                        x = DT == DLLM_DTYPE_BF16 ? __uint_as_float((uint32_t)u << 16)
-                                                  : __half2float(__ushort_as_half(u));
-                    }
-                }
-                f[e] = x;
-            }
+            x[i] = (x[i] & keep) | (Vec<DT>::NINF & ~keep);
         }
+        return make_uint4(x[0], x[1], x[2], x[3]);
     };
 
     float m = -INFINITY;   // this thread's maximum so far
     double s = 0.0;        // sum of exp(x - m)
-    uint32_t thr = KEY_NINF + 1;  // a candidate's key has to reach it
-    bool first_tile = true;
-    float x[E];
+    uint32_t thr = KEY_NINF + 1;   // a candidate's key has to reach it
+    int count = 0;                 // candidates in this warp's buffer
+    uint64_t *mine = buf + wid * BS_WCAP;
 
-    auto append = [&](int64_t j, int u) {
-#pragma unroll
-        for (int e = 0; e < VEC; e++) {
-            const uint32_t key = okey(x[u * VEC + e]);
-            if (x[u * VEC + e] == x[u * VEC + e] && key >= thr) {
-                const int at = atomicAdd(&count, 1);
-                if (at < BS_CAP) buf[at] = composite(key, (int)(j * VEC - shift + e));
-            }
-        }
-    };
-    // sorts the buffer, keeps the k best; the threshold is then above the last one kept
+    // this warp's k best, sorted
     auto cut = [&]() {
-        const int n = count;
-        sort_desc(buf, n, pow2_at_least(n));
-        if (n >= k) thr = max(thr, (uint32_t)(buf[k - 1] >> 32) + 1);
-        __syncthreads();
-        if (tid == 0) count = n < k ? n : k;
-        __syncthreads();
+        for (int i = count + lane; i < BS_WCAP; i += 32) mine[i] = 0;
+        __syncwarp();
+        sort_desc(mine, BS_WCAP, lane, 32, [] { __syncwarp(); });
+        if (count >= k) {
+            count = k;
+            const uint32_t last = (uint32_t)(mine[k - 1] >> 32);
+            if (lane == 0) atomicMax(&floor_key, last);
+            thr = max(thr, last + 1);
+        }
+        __syncwarp();
     };
 
-    for (int64_t t0 = v0; t0 < v1; t0 += (int64_t)BS_NT * BS_U) {
+    uint4 x[BS_U], next[BS_U];
 #pragma unroll
-        for (int u = 0; u < BS_U; u++) load(t0 + (int64_t)u * BS_NT + tid, x + u * VEC);
-        float tm = x[0];
+    for (int u = 0; u < BS_U; u++) next[u] = load(v0 + u * BS_NT + tid);
+    bool first_tile = true;
+    for (int t0 = v0; t0 < v1; t0 += BS_NT * BS_U) {
+        float vm[BS_U];
 #pragma unroll
-        for (int e = 1; e < E; e++) tm = fmaxf(tm, x[e]);
-        const float mn = fmaxf(m, tm), ref = mn == -INFINITY ? 0.0f : mn;
-        float part = 0.0f;
+        for (int u = 0; u < BS_U; u++) x[u] = next[u];
 #pragma unroll
-        for (int e = 0; e < E; e++) part += exp2_approx((x[e] - ref) * LOG2E);
+        for (int u = 0; u < BS_U; u++) next[u] = load(t0 + (BS_U + u) * BS_NT + tid);
+        float tm = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < BS_U; u++) {
+            vm[u] = vec_max<DT>(x[u]);
+            tm = max_keep(tm, vm[u]);
+        }
+        const float mn = max_keep(m, tm), ref = mn == -INFINITY ? 0.0f : mn;
+        float2 part = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int u = 0; u < BS_U; u++)
+#pragma unroll
+            for (int i = 0; i < VEC / 2; i++) {
+                const float2 y = mul2(add2(pair_of<DT>(x[u], i), make_float2(-ref, -ref)), make_float2(LOG2E, LOG2E));
+                part = add2(part, make_float2(exp2_approx(y.x), exp2_approx(y.y)));
+            }
         if (mn != m) s *= (double)exp2_approx((m - ref) * LOG2E);
         m = mn;
-        s += (double)part;
+        s += (double)(part.x + part.y);
 
-        uint32_t lo = KEY_NINF;  // first tile: a key that k of its entries reach
-        if (first_tile) {
-            const uint32_t kj = warp_jth(okey(tm), (k + BS_WARPS - 1) / BS_WARPS);
+        if (first_tile) {  // the first threshold, from every warp's first tile
+            const uint32_t kj = warp_jth(okey(m), jth);
             if (lane == 0) wkey[wid] = kj;
             __syncthreads();
-            lo = wkey[0];
+            first_tile = false;
+        }
+        if (__any_sync(0xffffffffu, okey(tm) >= thr)) {
+            const uint32_t kj = warp_jth(okey(m), jth);
+            if (lane == 0) wkey[wid] = kj;
+            __syncwarp();
+            uint32_t lo = wkey[0];
 #pragma unroll
             for (int w = 1; w < BS_WARPS; w++) lo = min(lo, wkey[w]);
-            thr = max(thr, lo);
-        }
-        const int before = count;
-        __syncthreads();
-        if (okey(tm) >= thr) {
-#pragma unroll
-            for (int u = 0; u < BS_U; u++) append(t0 + (int64_t)u * BS_NT + tid, u);
-        }
-        __syncthreads();
-        if (count > BS_CAP) {  // too many at once: take the tile again, a vector of each thread at a time
-            __syncthreads();
-            if (tid == 0) count = before;
+            thr = max(thr, max(lo, *(volatile uint32_t *)&floor_key));
 #pragma unroll
             for (int u = 0; u < BS_U; u++) {
-                __syncthreads();
-                const int held = count;
-                __syncthreads();
-                if (held > BS_CAP - BS_NT * VEC) cut();
-                append(t0 + (int64_t)u * BS_NT + tid, u);
+                if (!__any_sync(0xffffffffu, okey(vm[u]) >= thr)) continue;
+                if (count > BS_WCAP - 32 * VEC) cut();
+                const int i0 = (t0 + u * BS_NT + tid) * VEC - shift;
+#pragma unroll
+                for (int e = 0; e < VEC; e++) {
+                    const float2 pr = pair_of<DT>(x[u], e / 2);
+                    const float f = e & 1 ? pr.y : pr.x;
+                    const uint32_t key = okey(f);
+                    const bool take = f == f && key >= thr;
+                    const uint32_t who = __ballot_sync(0xffffffffu, take);
+                    if (take) mine[count + __popc(who & ((1u << lane) - 1))] = composite(key, i0 + e);
+                    count += __popc(who);
+                }
             }
-            __syncthreads();
         }
-        if (lo > KEY_NINF) thr = max(thr, lo + 1);
-        first_tile = false;
-        const int held = count;
-        __syncthreads();
-        if (held > BS_CAP / 2) cut();
     }
 
-    // the chunk's maximum and sum
+    // the chunk's maximum and sum, and the warps' candidates that reach the last threshold
     float M = m;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    if (lane == 0) wm[wid] = M;
+    for (int o = 16; o; o >>= 1) M = max_keep(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const uint32_t kj = warp_jth(okey(m), jth);
+    if (lane == 0) {
+        wm[wid] = M;
+        wkey[wid] = kj;
+        wcount[wid] = 0;
+    }
     __syncthreads();
+    uint32_t lo = wkey[0];
 #pragma unroll
-    for (int w = 0; w < BS_WARPS; w++) M = fmaxf(M, wm[w]);
+    for (int w = 0; w < BS_WARPS; w++) {
+        M = max_keep(M, wm[w]);
+        lo = min(lo, wkey[w]);
+    }
     const float ref = M == -INFINITY ? 0.0f : M;
     double S = m == -INFINITY ? s : s * (double)expf(m - ref);
 #pragma unroll
     for (int o = 16; o; o >>= 1) S += __shfl_xor_sync(0xffffffffu, S, o);
-    if (lane == 0) ws[wid] = S;
-    const int n = count;
-    sort_desc(buf, n, pow2_at_least(n));
+    const uint64_t lowest = (uint64_t)max(lo, floor_key) << 32;
+    int kept = 0;
+    for (int i = lane; i < (count + 31) / 32 * 32; i += 32) {  // in place: what is kept moves towards the front
+        const uint64_t c = i < count ? mine[i] : 0;
+        const bool keep = i < count && c >= lowest;
+        const uint32_t who = __ballot_sync(0xffffffffu, keep);
+        if (keep) mine[kept + __popc(who & ((1u << lane) - 1))] = c;
+        kept += __popc(who);
+    }
+    if (lane == 0) {
+        ws[wid] = S;
+        wcount[wid] = kept;
+    }
+    __syncthreads();
+    int n = 0, at = 0;
+#pragma unroll
+    for (int w = 0; w < BS_WARPS; w++) {
+        if (w == wid) at = n;
+        n += wcount[w];
+    }
     const int64_t chunk = blockIdx.x;
     if (tid == 0) {
         double tot = 0.0;
         for (int w = 0; w < BS_WARPS; w++) tot += ws[w];
         sums[chunk] = {M, 0.0f, tot};
     }
-    for (int i = tid; i < k; i += BS_NT) cands[chunk * k + i] = i < n ? buf[i] : 0;
+    uint64_t *out = cands + chunk * k;
+    if (n <= BS_NT) {  // each candidate's place is the number of larger ones
+        for (int i = lane; i < kept; i += 32) few[at + i] = mine[i];
+        __syncthreads();
+        if (tid < n) {
+            const uint64_t c = few[tid];
+            int place = 0;
+            for (int i = 0; i < n; i++) place += few[i] > c;
+            if (place < k) out[place] = c;
+        }
+        for (int i = n + tid; i < k; i += BS_NT) out[i] = 0;
+        return;
+    }
+    for (int i = kept + lane; i < BS_WCAP; i += 32) mine[i] = 0;
+    __syncthreads();
+    sort_desc(buf, BS_CAP, tid, BS_NT, [] { __syncthreads(); });
+    for (int i = tid; i < k; i += BS_NT) out[i] = buf[i];
 }
 
 struct Best {
@@ -296,8 +395,14 @@ __device__ __forceinline__ bool before(const Best &a, const Best &b) {
     return a.comp > b.comp;
 }
 
-// One CTA per sequence: the beams' log-sum-exps from their chunks, then k rounds, each taking the
-// best candidate that comes after the one taken last.
+// One CTA per sequence: the beams' log-sum-exps from their chunks, then the k best of the chunks'
+// candidates.  The same threshold as in a chunk (over the threads' best ranks, rounded down to
+// fp32, which keeps their order) leaves a few; each one's place is the number that comes before
+// it.  Where more are left than fit, the threshold is raised to the highest that k candidates
+// reach; where that still leaves too many (equal ranks), k rounds take the best candidate that
+// comes after the one taken last.
+constexpr int BM_LEFT = 512;
+
 __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, const ChunkSum *sums,
                                                            const uint64_t *cands, int chunks) {
     __shared__ double lse[DLLM_BEAM_MAX], inv_len[DLLM_BEAM_MAX];
@@ -305,62 +410,150 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
     __shared__ int length_in[DLLM_BEAM_MAX];
     __shared__ int live[DLLM_BEAM_MAX];  // 0 nothing to offer, 1 its row's continuations, 2 ended
     __shared__ Best wbest[BS_WARPS];
+    __shared__ Best left[BM_LEFT];
+    __shared__ uint32_t wkey[BS_WARPS];
+    __shared__ int nleft;
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const int K = d.beams, k = d.k;
     const int64_t item = blockIdx.x;
-    for (int b = tid; b < K; b += BS_NT) {
+    if (tid == 0) nleft = 0;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int b = wid; b < K; b += BS_WARPS) {
         const int64_t row = item * K + b;
         const float sc = d.scores[row];
         const bool ended = d.finished && d.finished[row];
+        const int len_in = d.lengths ? d.lengths[row] : 0;
         int st = 0, kind = 0;
         double l = 0.0;
         if (sc != sc || sc == INFINITY) st = DLLM_ROW_ERR_NONFINITE;
         else if (ended) kind = sc >= -FLT_MAX ? 2 : 0;
         else if (sc >= -FLT_MAX) {
             float M = -INFINITY;
-            for (int c = 0; c < chunks; c++) M = fmaxf(M, sums[row * chunks + c].m);
+            for (int c = lane; c < chunks; c += 32) M = max_keep(M, sums[row * chunks + c].m);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) M = max_keep(M, __shfl_xor_sync(0xffffffffu, M, o));
             double S = 0.0;
-            for (int c = 0; c < chunks; c++) {
+            for (int c = lane; c < chunks; c += 32) {
                 const ChunkSum p = sums[row * chunks + c];
-                S += p.m == -INFINITY ? p.s : p.s * exp((double)p.m - (double)M);
+                S += p.m == -INFINITY || p.m == M ? p.s : p.s * exp((double)p.m - (double)M);
             }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) S += __shfl_xor_sync(0xffffffffu, S, o);
             if (S != S || M == INFINITY) st = DLLM_ROW_ERR_NONFINITE;
             else if (M > -INFINITY) {
                 kind = 1;
                 l = (double)M + log(S);
             }
         }
-        length_in[b] = d.lengths ? d.lengths[row] : 0;
-        const double len = fmax((double)length_in[b] + (ended ? 0.0 : 1.0), 1.0);
-        score_in[b] = sc;
-        lse[b] = l;
-        inv_len[b] = d.length_penalty != 0.0f && d.lengths ? 1.0 / pow(len, (double)d.length_penalty) : 1.0;
-        live[b] = kind;
-        if (d.status) d.status[row] = st;
+        if (lane == 0) {
+            const double len = fmax((double)len_in + (ended ? 0.0 : 1.0), 1.0);
+            length_in[b] = len_in;
+            score_in[b] = sc;
+            lse[b] = l;
+            inv_len[b] = d.length_penalty != 0.0f && d.lengths ? 1.0 / pow(len, (double)d.length_penalty) : 1.0;
+            live[b] = kind;
+            if (d.status) d.status[row] = st;
+        }
     }
     __syncthreads();
-    const int64_t N = (int64_t)K * chunks * k;
+    const int per_beam = chunks * k, N = K * per_beam;
+    const uint64_t *mine = cands + item * N;
     // candidate e: position e % k of a chunk's list; an ended beam offers its first position only
-    auto candidate = [&](int64_t e, Best *c) {
-        const int b = (int)(e / ((int64_t)chunks * k));
+    auto candidate = [&](int e, Best *c) {
+        const int b = e / per_beam;
         if (live[b] == 0) return false;
         double cum = (double)score_in[b];
         uint64_t comp;
         if (live[b] == 2) {
-            if (e % ((int64_t)chunks * k)) return false;
+            if (e != b * per_beam) return false;
             comp = composite(0, d.eos);
         } else {
-            comp = cands[item * N + e];
+            comp = mine[e];
             if (!comp) return false;
             cum += (double)okey_value((uint32_t)(comp >> 32)) - lse[b];
         }
         *c = {cum * inv_len[b], b, comp};
         return true;
     };
+    auto emit = [&](int place, const Best &c, bool none) {
+        float score = -INFINITY;
+        if (!none) {
+            double cum = (double)score_in[c.beam];
+            if (live[c.beam] == 1) cum += (double)okey_value((uint32_t)(c.comp >> 32)) - lse[c.beam];
+            score = __double2float_rn(cum);
+        }
+        d.out_score[item * k + place] = score;
+        d.out_parent[item * k + place] = none ? -1 : c.beam;
+        const int32_t token = none ? -1 : (int32_t)~(uint32_t)c.comp;
+        const bool ended = !none && live[c.beam] == 2;
+        d.out_token[item * k + place] = token;
+        if (d.out_finished) d.out_finished[item * k + place] = ended || (!none && token == d.eos);
+        if (d.out_lengths) d.out_lengths[item * k + place] = none ? 0 : length_in[c.beam] + (ended ? 0 : 1);
+    };
+    uint32_t mx = 0;
+    for (int e = tid; e < N; e += BS_NT) {
+        Best c;
+        if (candidate(e, &c)) mx = max(mx, okey(__double2float_rd(c.rank)));
+    }
+    const uint32_t kj = warp_jth(mx, (k + BS_WARPS - 1) / BS_WARPS);
+    if (lane == 0) wkey[wid] = kj;
+    __syncthreads();
+    uint32_t lo = wkey[0];
+#pragma unroll
+    for (int w = 1; w < BS_WARPS; w++) lo = min(lo, wkey[w]);
+    for (int e = tid; e < N; e += BS_NT) {
+        Best c;
+        if (!candidate(e, &c) || okey(__double2float_rd(c.rank)) < lo) continue;
+        const int at = atomicAdd(&nleft, 1);
+        if (at < BM_LEFT) left[at] = c;
+    }
+    __syncthreads();
+    int n = nleft;
+    if (n > BM_LEFT) {  // the largest threshold that k candidates reach, by bisection of its key
+        uint32_t reached = lo, above = 0xffffffffu;
+        while (above - reached > 1) {
+            const uint32_t mid = reached + (above - reached) / 2;
+            int c_mid = 0;
+            for (int e = tid; e < N; e += BS_NT) {
+                Best c;
+                c_mid += candidate(e, &c) && okey(__double2float_rd(c.rank)) >= mid;
+            }
+            c_mid = __reduce_add_sync(0xffffffffu, c_mid);
+            __syncthreads();
+            if (lane == 0) wkey[wid] = c_mid;
+            __syncthreads();
+            c_mid = 0;
+#pragma unroll
+            for (int w = 0; w < BS_WARPS; w++) c_mid += wkey[w];
+            if (c_mid >= k) reached = mid;
+            else above = mid;
+        }
+        __syncthreads();
+        if (tid == 0) nleft = 0;
+        __syncthreads();
+        for (int e = tid; e < N; e += BS_NT) {
+            Best c;
+            if (!candidate(e, &c) || okey(__double2float_rd(c.rank)) < reached) continue;
+            const int at = atomicAdd(&nleft, 1);
+            if (at < BM_LEFT) left[at] = c;
+        }
+        __syncthreads();
+        n = nleft;
+    }
+    if (n <= BM_LEFT) {
+        for (int i = tid; i < n; i += BS_NT) {
+            const Best c = left[i];
+            int place = 0;
+            for (int j = 0; j < n; j++) place += before(left[j], c);
+            if (place < k) emit(place, c, false);
+        }
+        for (int i = n + tid; i < k; i += BS_NT) emit(i, Best{}, true);
+        return;
+    }
     Best last = {INFINITY, -1, 0};
     for (int r = 0; r < k; r++) {
         Best best = {-INFINITY, 1 << 30, 0};
-        for (int64_t e = tid; e < N; e += BS_NT) {
+        for (int e = tid; e < N; e += BS_NT) {
             Best c;
             if (candidate(e, &c) && before(last, c) && before(c, best)) best = c;
         }
@@ -377,33 +570,26 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
         for (int w = 1; w < BS_WARPS; w++)
             if (before(wbest[w], best)) best = wbest[w];
         __syncthreads();
-        const bool none = best.beam == 1 << 30;
-        if (tid == 0) {
-            float score = -INFINITY;
-            if (!none) {
-                double cum = (double)score_in[best.beam];
-                if (live[best.beam] == 1) cum += (double)okey_value((uint32_t)(best.comp >> 32)) - lse[best.beam];
-                score = __double2float_rn(cum);
-            }
-            d.out_score[item * k + r] = score;
-            d.out_parent[item * k + r] = none ? -1 : best.beam;
-            const int32_t token = none ? -1 : (int32_t)~(uint32_t)best.comp;
-            const bool ended = !none && live[best.beam] == 2;
-            d.out_token[item * k + r] = token;
-            if (d.out_finished) d.out_finished[item * k + r] = ended || (!none && token == d.eos);
-            if (d.out_lengths) d.out_lengths[item * k + r] = none ? 0 : length_in[best.beam] + (ended ? 0 : 1);
-        }
-        last = none ? Best{-INFINITY, 1 << 30, 0} : best;
+        if (tid == 0) emit(r, best, false);  // more candidates than BM_LEFT >= k: there is one
+        last = best;
     }
 }
 
-// Chunks per row: enough CTAs to fill the GPU, no chunk smaller than one tile.
+// Chunks per row: the count whose waves of CTAs (4 per SM) take least, a chunk's set-up and
+// selection counted as two tiles.
 int beam_chunks(int64_t rows, int vocab, int dtype) {
     const int vec = dtype == DLLM_DTYPE_F32 ? 4 : 8;
-    const int64_t tile = (int64_t)BS_NT * BS_U * vec;
-    int64_t most = (vocab + tile - 1) / tile, want = (148 * 6 + rows - 1) / rows;
-    if (want > most) want = most;
-    return (int)(want < 1 ? 1 : want);
+    const int64_t tiles = ((int64_t)vocab + BS_NT * BS_U * vec - 1) / (BS_NT * BS_U * vec), slots = 148 * 4;
+    int best = 1;
+    int64_t least = INT64_MAX;
+    for (int c = 1; c <= tiles && c <= 64; c++) {
+        const int64_t cost = (rows * c + slots - 1) / slots * ((tiles + c - 1) / c + 2);
+        if (cost < least) {
+            least = cost;
+            best = c;
+        }
+    }
+    return best;
 }
 
 // ----------------------------------------------------------------------------------------
@@ -498,8 +684,20 @@ dllm_status launch_beam_select(const dllm_beam_desc *d, void *ws, cudaStream_t s
         else go(beam_chunk_kernel<DLLM_DTYPE_F16, false>);
     }
     if (cudaGetLastError() != cudaSuccess) return DLLM_ERR_CUDA;
-    beam_merge_kernel<<<d->batch, BS_NT, 0, stream>>>(*d, sums, cands, chunks);
-    return cudaGetLastError() == cudaSuccess ? DLLM_OK : DLLM_ERR_CUDA;
+    // launched while the chunks run; it waits for them on the GPU
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(d->batch);
+    cfg.blockDim = dim3(BS_NT);
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, beam_merge_kernel, *d, (const ChunkSum *)sums, (const uint64_t *)cands, chunks) ==
+                   cudaSuccess
+               ? DLLM_OK
+               : DLLM_ERR_CUDA;
 }
 
 dllm_status launch_beam_reorder(int batch, int beams, const int32_t *parent, int ntensors, void *const *tensors,
