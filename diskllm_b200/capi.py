@@ -686,6 +686,9 @@ def lmhead_logits(h, w, *, norm_w=None, eps=1e-6, add_one=False, softcap=0.0, lo
 
 
 # ---- int8 LM head -----------------------------------------------------------------------------
+#
+# These calls serve decode steps of a few microseconds, so their checks are written to cost little:
+# messages are only formatted where a check fails, and devices are compared by index.
 
 _FLOATS = None
 
@@ -700,45 +703,66 @@ def _float_code(dtype):
     return _FLOATS.get(dtype)
 
 
-def _need(ok, what):
-    if not ok:
-        raise DllmError(what)
-
-
 def _vector(t, n, dtype, dev, name):
-    """A contiguous device vector of n elements."""
-    _need(t.dtype == dtype and t.device == dev and t.is_contiguous() and t.numel() == n,
-          f"{name}: a contiguous {dtype} tensor of {n} elements on {dev} is needed")
+    """Pointer of a contiguous vector of n elements on device `dev` (an index)."""
+    if t.dtype is not dtype or t.get_device() != dev or t.numel() != n or not t.is_contiguous():
+        raise DllmError(f"{name}: a contiguous {dtype} tensor of {n} elements on cuda:{dev} is needed")
     return t.data_ptr()
+
+
+def _flags(t, n, dev, name):
+    """Pointer of n contiguous bytes used as truth values."""
+    import torch
+
+    return _vector(t, n, torch.bool if t.dtype is torch.bool else torch.uint8, dev, name)
 
 
 def _codes(t, dev, name):
     """(pointer, rows, cols, stride) of int8 rows that start on multiples of 16 bytes."""
     import torch
 
-    _need(t.dtype == torch.int8 and t.device == dev and t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] <= 1),
-          f"{name}: int8 rows on {dev} are needed")
+    if t.dtype is not torch.int8 or t.get_device() != dev or t.dim() != 2:
+        raise DllmError(f"{name}: int8 rows on cuda:{dev} are needed")
     rows, cols = t.shape
-    stride = t.stride(0)
+    stride, inner = t.stride()
     if rows <= 1:  # the stride of a single row is not used
         stride = (cols + 15) // 16 * 16
-    _need(t.data_ptr() % 16 == 0 and stride % 16 == 0 and stride >= cols,
-          f"{name}: rows have to start on multiples of 16 bytes (quantize_rows_i8 lays them out so)")
-    return t.data_ptr(), rows, cols, stride
+    ptr = t.data_ptr()
+    if (inner != 1 and cols > 1) or ptr % 16 or stride % 16 or stride < cols:
+        raise DllmError(f"{name}: contiguous rows that start on multiples of 16 bytes are needed "
+                        "(quantize_rows_i8 lays them out so)")
+    return ptr, rows, cols, stride
+
+
+def _scratch(ws, dev):
+    """(pointer, bytes) of a workspace."""
+    if ws.get_device() != dev or not ws.is_contiguous():
+        raise DllmError(f"workspace: a contiguous tensor on cuda:{dev} is needed")
+    return ws.data_ptr(), ws.numel() * ws.element_size()
+
+
+_torch_c = None
 
 
 def _call(name, dev, stream, *args):
-    """Runs a library call on `stream` (default: the current one of `dev`), with `dev` current."""
-    import torch
+    """Runs a library call on `stream` (default: the current one of device `dev`), with `dev` current."""
+    global _torch_c
+    if _torch_c is None:
+        import torch
 
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # without making a Stream object
+        _torch_c = (raw or (lambda i: torch.cuda.current_stream(i).cuda_stream), torch.cuda.current_device,
+                    torch.cuda.device)
     if stream is None:
-        stream = torch.cuda.current_stream(dev).cuda_stream
+        stream = _torch_c[0](dev)
     f = getattr(load_library(), name)
-    if torch.cuda.current_device() == dev.index:
-        _check(f(*args, stream), name)
+    if _torch_c[1]() == dev:
+        rc = f(*args, stream)
     else:
-        with torch.cuda.device(dev):
-            _check(f(*args, stream), name)
+        with _torch_c[2](dev):
+            rc = f(*args, stream)
+    if rc != DLLM_OK:
+        _check(rc, name)
 
 
 def quantize_rows_i8(x, *, norm=False, norm_w=None, eps=1e-6, add_one=False, q=None, scale=None, stream=None):
@@ -747,21 +771,28 @@ def quantize_rows_i8(x, *, norm=False, norm_w=None, eps=1e-6, add_one=False, q=N
     codes' rows start on multiples of 16 bytes."""
     import torch
 
-    code = _float_code(x.dtype)
-    _need(x.is_cuda and x.dim() == 2 and code is not None, "x: a 2-D fp32, bf16 or fp16 CUDA tensor is needed")
+    code, dev = _float_code(x.dtype), x.get_device()
+    if dev < 0 or x.dim() != 2 or code is None:
+        raise DllmError("x: a 2-D fp32, bf16 or fp16 CUDA tensor is needed")
     rows, cols = x.shape
-    _need(cols >= 1 and (x.stride(1) == 1 or cols == 1), "x: rows of at least one element, contiguous")
-    dev = x.device
+    x_stride, inner = x.stride()
+    if cols < 1 or (inner != 1 and cols > 1):
+        raise DllmError("x: contiguous rows of at least one element are needed")
     if q is None:
-        q = torch.empty(rows, (cols + 15) // 16 * 16, dtype=torch.int8, device=dev)[:, :cols]
+        ld = (cols + 15) // 16 * 16
+        q = torch.empty((rows, ld), dtype=torch.int8, device=x.device)
+        qp = q.data_ptr()
+        if ld != cols:
+            q = q[:, :cols]
+    else:
+        qp, qr, qc, ld = _codes(q, dev, "q")
+        if (qr, qc) != (rows, cols):
+            raise DllmError("q: the shape of x is needed")
     if scale is None:
-        scale = torch.empty(rows, dtype=torch.float32, device=dev)
-    qp, qr, qc, qs = _codes(q, dev, "q")
-    _need((qr, qc) == (rows, cols), "q: the shape of x is needed")
-    wp = None if norm_w is None else _vector(norm_w, cols, torch.float32, dev, "norm_w")
-    _call("dllm_cuda_quantize_rows_i8", dev, stream, rows, cols, x.data_ptr(), max(x.stride(0), cols) if rows <= 1 else
-          x.stride(0), code, int(bool(norm)), wp, float(eps), int(bool(add_one)), qp, qs,
-          _vector(scale, rows, torch.float32, dev, "scale"))
+        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    _call("dllm_cuda_quantize_rows_i8", dev, stream, rows, cols, x.data_ptr(), x_stride if rows > 1 else cols, code,
+          bool(norm), None if norm_w is None else _vector(norm_w, cols, torch.float32, dev, "norm_w"), eps, bool(add_one),
+          qp, ld, _vector(scale, rows, torch.float32, dev, "scale"))
     return q, scale
 
 
@@ -770,19 +801,26 @@ def matmul_i8(a, a_scale, b, b_scale, *, softcap=0.0, out=None, out_dtype=None, 
     [m][k], b [n][k] as quantize_rows_i8 gives them, fp32 scales; out fp32 (default), bf16 or fp16."""
     import torch
 
-    _need(a.is_cuda, "a: a CUDA tensor is needed")
-    dev = a.device
+    dev = a.get_device()
+    if dev < 0:
+        raise DllmError("a: a CUDA tensor is needed")
     ap, m, k, lda = _codes(a, dev, "a")
     bp, n, kb, ldb = _codes(b, dev, "b")
-    _need(k == kb, f"a has {k} columns, b {kb}")
+    if k != kb:
+        raise DllmError(f"a has {k} columns, b {kb}")
     if out is None:
-        out = torch.empty(m, n, dtype=out_dtype or torch.float32, device=dev)
-    code = _float_code(out.dtype)
-    _need(code is not None and out.device == dev and out.shape == (m, n) and (n <= 1 or out.stride(1) == 1)
-          and (out_dtype is None or out.dtype == out_dtype), "out: rows [m][n] of fp32, bf16 or fp16 are needed")
+        out = torch.empty((m, n), dtype=out_dtype or torch.float32, device=a.device)
+        code, ldo = _float_code(out.dtype), n
+    else:
+        code = _float_code(out.dtype)
+        if out.get_device() != dev or out.shape != (m, n) or (n > 1 and out.stride(1) != 1) or \
+                (out_dtype is not None and out.dtype is not out_dtype):
+            raise DllmError(f"out: contiguous rows [{m}][{n}] are needed")
+        ldo = out.stride(0) if m > 1 else n
+    if code is None:
+        raise DllmError("out: fp32, bf16 or fp16 is needed")
     _call("dllm_cuda_matmul_i8", dev, stream, m, n, k, ap, lda, _vector(a_scale, m, torch.float32, dev, "a_scale"), bp,
-          ldb, _vector(b_scale, n, torch.float32, dev, "b_scale"), float(softcap), out.data_ptr(),
-          out.stride(0) if m > 1 else max(out.stride(0), n), code,
+          ldb, _vector(b_scale, n, torch.float32, dev, "b_scale"), softcap, out.data_ptr(), ldo, code,
           None if status is None else _vector(status, 1, torch.int32, dev, "status"))
     return out
 
@@ -793,24 +831,23 @@ def lmhead_logits_i8(h, w, w_scale, *, norm_w=None, eps=1e-6, add_one=False, sof
     [vocab][hidden] and w_scale fp32 [vocab] from quantize_rows_i8; returns fp32 logits [rows][vocab]."""
     import torch
 
-    _need(h.is_cuda and h.dim() == 2 and h.dtype == torch.float32 and h.is_contiguous(),
-          "h: a contiguous fp32 [rows][hidden] CUDA tensor is needed")
-    dev = h.device
+    dev = h.get_device()
+    if dev < 0 or h.dim() != 2 or h.dtype is not torch.float32 or not h.is_contiguous():
+        raise DllmError("h: a contiguous fp32 [rows][hidden] CUDA tensor is needed")
     rows, hidden = h.shape
     wp, vocab, hw, ldw = _codes(w, dev, "w")
-    _need(hidden == hw, f"h has {hidden} columns, w {hw}")
+    if hidden != hw:
+        raise DllmError(f"h has {hidden} columns, w {hw}")
     if logits is None:
-        logits = torch.empty(rows, vocab, dtype=torch.float32, device=dev)
+        logits = torch.empty((rows, vocab), dtype=torch.float32, device=h.device)
     if workspace is None:
         workspace = torch.empty(load_library().dllm_cuda_lmhead_i8_workspace_bytes(rows, hidden), dtype=torch.uint8,
-                                device=dev)
-    _need(workspace.device == dev and workspace.is_contiguous(), f"workspace: contiguous, on {dev}")
+                                device=h.device)
     _call("dllm_cuda_lmhead_logits_i8", dev, stream, rows, hidden, vocab, h.data_ptr(),
-          None if norm_w is None else _vector(norm_w, hidden, torch.float32, dev, "norm_w"), float(eps),
-          int(bool(add_one)), wp, ldw, _vector(w_scale, vocab, torch.float32, dev, "w_scale"), float(softcap),
+          None if norm_w is None else _vector(norm_w, hidden, torch.float32, dev, "norm_w"), eps, bool(add_one), wp, ldw,
+          _vector(w_scale, vocab, torch.float32, dev, "w_scale"), softcap,
           _vector(logits, rows * vocab, torch.float32, dev, "logits"),
-          None if status is None else _vector(status, 1, torch.int32, dev, "status"), workspace.data_ptr(),
-          workspace.numel() * workspace.element_size())
+          None if status is None else _vector(status, 1, torch.int32, dev, "status"), *_scratch(workspace, dev))
     return logits
 
 
@@ -821,52 +858,46 @@ def fill_beam_desc(logits, scores, k, *, mask=None, finished=None, eos=-1, lengt
     """Builds a dllm_beam_desc from CUDA tensors; returns (desc, (score, parent, token), workspace)."""
     import torch
 
-    code = _float_code(logits.dtype)
-    _need(logits.is_cuda and logits.dim() == 2 and code is not None,
-          "logits: a 2-D fp32, bf16 or fp16 CUDA tensor is needed")
-    dev = logits.device
-    _need(scores.dim() == 2, "scores: [batch][beams] is needed")
+    code, dev = _float_code(logits.dtype), logits.get_device()
+    if dev < 0 or logits.dim() != 2 or code is None:
+        raise DllmError("logits: a 2-D fp32, bf16 or fp16 CUDA tensor is needed")
+    if scores.dim() != 2:
+        raise DllmError("scores: [batch][beams] is needed")
     batch, beams = scores.shape
     rows, vocab = logits.shape
-    _need(rows == batch * beams, f"logits have {rows} rows, scores {batch} x {beams}")
-    _need(vocab <= 1 or logits.stride(1) == 1, "logits: contiguous rows are needed")
+    row_stride, inner = logits.stride()
+    if rows != batch * beams:
+        raise DllmError(f"logits have {rows} rows, scores {batch} x {beams}")
+    if vocab > 1 and inner != 1:
+        raise DllmError("logits: contiguous rows are needed")
     k = int(k)
-    d = BeamDesc()
-    d.batch, d.beams, d.vocab, d.k, d.dtype = batch, beams, vocab, k, code
-    d.row_stride = logits.stride(0) if rows > 1 else max(logits.stride(0), vocab)
-    d.logits = logits.data_ptr()
-    d.scores = _vector(scores, rows, torch.float32, dev, "scores")
+    n = batch * k
+    mask_ptr = mask_stride = 0
     if mask is not None:
-        _need(mask.dtype in (torch.int32, torch.uint32) and mask.device == dev and mask.dim() == 2
-              and mask.shape[0] == rows and mask.shape[1] >= (vocab + 31) // 32
-              and (mask.stride(1) == 1 or mask.shape[1] == 1), "mask: int32 words [rows][(vocab + 31) / 32] are needed")
-        d.mask, d.mask_stride = mask.data_ptr(), mask.stride(0) if rows > 1 else max(mask.stride(0), mask.shape[1])
-    if finished is not None:
-        _need(finished.dtype in (torch.uint8, torch.bool), "finished: uint8 or bool is needed")
-        d.finished = _vector(finished, rows, finished.dtype, dev, "finished")
-    d.eos = int(eos)
-    if lengths is not None:
-        d.lengths = _vector(lengths, rows, torch.int32, dev, "lengths")
-    d.length_penalty = float(length_penalty)
+        words = (vocab + 31) // 32
+        if mask.dtype not in (torch.int32, torch.uint32) or mask.get_device() != dev or mask.dim() != 2 or \
+                mask.shape[0] != rows or mask.shape[1] < words or (mask.shape[1] > 1 and mask.stride(1) != 1):
+            raise DllmError(f"mask: int32 words [{rows}][{words}] on cuda:{dev} are needed")
+        mask_ptr, mask_stride = mask.data_ptr(), mask.stride(0) if rows > 1 else words
     if out is None:
-        buf = torch.empty(3, batch, max(k, 0), dtype=torch.int32, device=dev)
-        out = (buf[0].view(torch.float32), buf[1], buf[2])
-    score, parent, token = out
-    d.out_score = _vector(score, batch * k, torch.float32, dev, "out score")
-    d.out_parent = _vector(parent, batch * k, torch.int32, dev, "out parent")
-    d.out_token = _vector(token, batch * k, torch.int32, dev, "out token")
-    if out_finished is not None:
-        _need(out_finished.dtype in (torch.uint8, torch.bool), "out_finished: uint8 or bool is needed")
-        d.out_finished = _vector(out_finished, batch * k, out_finished.dtype, dev, "out_finished")
-    if out_lengths is not None:
-        d.out_lengths = _vector(out_lengths, batch * k, torch.int32, dev, "out_lengths")
-    if status is not None:
-        d.status = _vector(status, rows, torch.int32, dev, "status")
+        score, parent, token = torch.empty((3, batch, max(k, 0)), dtype=torch.int32, device=logits.device).unbind(0)
+        score = score.view(torch.float32)
+        out = (score, parent, token)
+    else:
+        score, parent, token = out
+    d = BeamDesc(batch, beams, vocab, k, row_stride if rows > 1 else vocab, code, logits.data_ptr(), mask_ptr, mask_stride,
+                 _vector(scores, rows, torch.float32, dev, "scores"),
+                 None if finished is None else _flags(finished, rows, dev, "finished"), int(eos),
+                 None if lengths is None else _vector(lengths, rows, torch.int32, dev, "lengths"), length_penalty,
+                 _vector(score, n, torch.float32, dev, "out score"), _vector(parent, n, torch.int32, dev, "out parent"),
+                 _vector(token, n, torch.int32, dev, "out token"),
+                 None if out_finished is None else _flags(out_finished, n, dev, "out_finished"),
+                 None if out_lengths is None else _vector(out_lengths, n, torch.int32, dev, "out_lengths"),
+                 None if status is None else _vector(status, rows, torch.int32, dev, "status"))
     if workspace is None:
         workspace = torch.empty(load_library().dllm_cuda_beam_workspace_bytes(C.byref(d)), dtype=torch.uint8,
-                                device=dev)
-    _need(workspace.device == dev and workspace.is_contiguous(), f"workspace: contiguous, on {dev}")
-    d.workspace, d.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+                                device=logits.device)
+    d.workspace, d.workspace_bytes = _scratch(workspace, dev)
     return d, out, workspace
 
 
@@ -877,26 +908,28 @@ def beam_select(logits, scores, k, *, stream=None, **kw):
     (packed allow-bits), `finished` and `eos` (ended beams), `lengths` and `length_penalty`, `out`
     (the three outputs), `out_finished`, `out_lengths`, `status`, `workspace`."""
     d, out, ws = fill_beam_desc(logits, scores, k, **kw)
-    _call("dllm_cuda_beam_select", logits.device, stream, C.byref(d))
+    _call("dllm_cuda_beam_select", logits.get_device(), stream, C.byref(d))
     return out
 
 
 def _runs(t):
-    """(row stride, segments, segment stride, run), the last three in bytes as the row stride, of a
-    state [rows][...] whose inner dimensions are runs of one length at one stride."""
+    """(row stride, segments, segment stride, run), strides and run in bytes, of a state [rows][...]
+    whose inner dimensions are runs of one length at one stride."""
     esz = t.element_size()
     run, segs, seg_stride = esz, 1, 0
-    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+    strides = t.stride()
+    for size, stride in zip(t.shape[:0:-1], strides[:0:-1]):
         if size == 1:
             continue
         if segs == 1 and stride * esz == run:
             run *= size
         elif segs == 1:
             segs, seg_stride = size, stride * esz
-        else:
-            _need(stride * esz == segs * seg_stride, "a state's rows have to be runs at one stride")
+        elif stride * esz == segs * seg_stride:
             segs *= size
-    return (t.stride(0) * esz, segs, seg_stride, run)
+        else:
+            raise DllmError("a state's rows have to be runs at one stride")
+    return strides[0] * esz, segs, seg_stride, run
 
 
 def beam_reorder(states, parents, *, stream=None):
@@ -906,17 +939,21 @@ def beam_reorder(states, parents, *, stream=None):
     without what lies around it."""
     import torch
 
-    _need(parents.is_cuda and parents.dim() == 2 and parents.dtype == torch.int32 and parents.is_contiguous(),
-          "parents: contiguous int32 [batch][beams] on the GPU is needed")
-    dev = parents.device
+    dev = parents.get_device()
+    if dev < 0 or parents.dim() != 2 or parents.dtype is not torch.int32 or not parents.is_contiguous():
+        raise DllmError("parents: contiguous int32 [batch][beams] on the GPU is needed")
     batch, beams = parents.shape
-    groups = {}
+    rows = batch * beams
+    groups, seen = {}, set()
     for t in states:
-        _need(t.device == dev and t.dim() >= 1 and t.shape[0] == batch * beams,
-              f"a state of {batch * beams} rows on {dev} is needed")
+        if t.get_device() != dev or t.dim() < 1 or t.shape[0] != rows:
+            raise DllmError(f"a state of {rows} rows on cuda:{dev} is needed")
         if t.numel():
-            groups.setdefault(_runs(t), []).append(t.data_ptr())
-    _need(len({p for ptrs in groups.values() for p in ptrs}) == sum(map(len, groups.values())), "a state is given twice")
+            ptr = t.data_ptr()
+            if ptr in seen:
+                raise DllmError("a state is given twice")
+            seen.add(ptr)
+            groups.setdefault(_runs(t), []).append(ptr)
     for (row, segs, seg, run), ptrs in groups.items():
         _call("dllm_cuda_beam_reorder", dev, stream, batch, beams, parents.data_ptr(), len(ptrs),
               (C.c_void_p * len(ptrs))(*ptrs), row, segs, seg, run)

@@ -25,7 +25,7 @@ constexpr int BS_WCAP = 512;        // candidates that a warp holds: at least k 
 constexpr int BS_CAP = BS_WARPS * BS_WCAP;
 constexpr uint32_t KEY_NINF = 0x007fffffu;  // order key of -inf
 
-// One chunk's maximum and exponential sum relative to it.
+// One chunk's maximum and its exponential sum, relative to sum_base(m).
 struct ChunkSum {
     float m;
     float pad;
@@ -52,20 +52,46 @@ __device__ __forceinline__ float max_keep(float a, float b) {
     asm("max.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
-// Two fp32 additions or products in one instruction.
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 y;
-    asm("{\n.reg .b64 a, b, y;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.ftz.f32x2 y, a, b;\nmov.b64 {%0, %1}, y;\n}"
-        : "=f"(y.x), "=f"(y.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+// Two fp32 values in a register pair, for the instructions that work on both.
+struct Pair {
+    unsigned long long v;
+    __device__ __forceinline__ Pair() {}
+    __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ float sum() const {
+        float a, b;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+        return a + b;
+    }
+};
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair y;
+    asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(y.v) : "l"(a.v), "l"(b.v));
     return y;
 }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 y;
-    asm("{\n.reg .b64 a, b, y;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.ftz.f32x2 y, a, b;\nmov.b64 {%0, %1}, y;\n}"
-        : "=f"(y.x), "=f"(y.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair y;
+    asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(y.v) : "l"(a.v), "l"(b.v), "l"(c.v));
     return y;
+}
+__device__ __forceinline__ Pair exp2_approx(Pair x) {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v));
+    return Pair(exp2_approx(a), exp2_approx(b));
+}
+
+// Exponential sums are held as sums of 2^(x * LOG2E - base(m)), m the largest x so far.  The base is
+// LOG2E * m rounded to fp32, so that one fused product-and-sum forms an exponent; from 2^20 on, where
+// that rounding is no longer small, it is the exact product and the exponent LOG2E * (x - m).
+// log(sum of e^x) is then (log2(sum) + base) / LOG2E with this LOG2E, whose own rounding (1.3e-8 of it)
+// changes the result by that much times the softmax's entropy.
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float BASE_EXACT = 1048576.0f;
+__device__ __forceinline__ double sum_base(float m) {
+    return fabsf(m) < BASE_EXACT ? (double)__fmul_rn(m, LOG2E) : (double)m * (double)LOG2E;
+}
+// what a sum relative to `from` is multiplied by to be one relative to `to` (>= from)
+__device__ __forceinline__ double rebase(float from, float to) {
+    return from == to ? 1.0 : from == -INFINITY ? 0.0 : (double)exp2_approx((float)(sum_base(from) - sum_base(to)));
 }
 
 // A candidate: (order key << 32) | ~id, so that a larger composite is (logit desc, id asc).
@@ -125,24 +151,71 @@ __device__ __forceinline__ float2 pair_of(const uint4 &v, int i) {
                        __half2float(__ushort_as_half((unsigned short)(u >> 16))));
 }
 
-// largest element of a vector
+// elementwise maximum of two words of 16-bit logits
 template <int DT>
-__device__ __forceinline__ float vec_max(const uint4 &v) {
-    if (DT == DLLM_DTYPE_F32)
-        return max_keep(max_keep(__uint_as_float(v.x), __uint_as_float(v.y)),
-                        max_keep(__uint_as_float(v.z), __uint_as_float(v.w)));
-    uint32_t a, b, c;
-    if (DT == DLLM_DTYPE_BF16) {
-        asm("max.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(v.x), "r"(v.y));
-        asm("max.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(v.z), "r"(v.w));
-        asm("max.bf16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
-    } else {
-        asm("max.f16x2 %0, %1, %2;" : "=r"(a) : "r"(v.x), "r"(v.y));
-        asm("max.f16x2 %0, %1, %2;" : "=r"(b) : "r"(v.z), "r"(v.w));
-        asm("max.f16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+__device__ __forceinline__ uint32_t max_words(uint32_t a, uint32_t b) {
+    uint32_t y;
+    if (DT == DLLM_DTYPE_BF16) asm("max.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+    else asm("max.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+    return y;
+}
+// the largest element of U vectors
+template <int DT, int U>
+__device__ __forceinline__ float largest(const uint4 (&v)[U]) {
+    if (DT == DLLM_DTYPE_F32) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            m = max_keep(m, max_keep(max_keep(__uint_as_float(v[u].x), __uint_as_float(v[u].y)),
+                                     max_keep(__uint_as_float(v[u].z), __uint_as_float(v[u].w))));
+        return m;
     }
-    const float2 p = pair_of<DT>(make_uint4(c, 0, 0, 0), 0);
+    uint32_t m = Vec<DT>::NINF;
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        m = max_words<DT>(m, max_words<DT>(max_words<DT>(v[u].x, v[u].y), max_words<DT>(v[u].z, v[u].w)));
+    const float2 p = pair_of<DT>(make_uint4(m, 0, 0, 0), 0);
     return max_keep(p.x, p.y);
+}
+
+// Which elements of U vectors are at or above `least`, as bits: element e of fp32 vectors at bit e;
+// of 16-bit ones, the lower element of word w at bit w and the upper one at bit 16 + w.  `least` is
+// rounded down to the type, so a few more may be marked.
+template <int DT, int U>
+__device__ __forceinline__ uint32_t reaching(const uint4 (&v)[U], float least) {
+    uint32_t take = 0;
+    if (DT == DLLM_DTYPE_F32) {
+#pragma unroll
+        for (int e = 0; e < 4 * U; e++) take |= (uint32_t)(__uint_as_float(word_of(v[e / 4], e % 4)) >= least) << e;
+        return take;
+    }
+    uint32_t two;  // -inf is never marked
+    if (DT == DLLM_DTYPE_BF16) two = __bfloat16_as_ushort(__float2bfloat16_rd(fmaxf(least, -3.38953139e38f)));
+    else two = __half_as_ushort(__float2half_rd(fmaxf(least, -65504.0f)));
+    two |= two << 16;
+#pragma unroll
+    for (int w = 0; w < 4 * U; w++) {
+        uint32_t ge;
+        if (DT == DLLM_DTYPE_BF16) asm("set.ge.u32.bf16x2 %0, %1, %2;" : "=r"(ge) : "r"(word_of(v[w / 4], w % 4)), "r"(two));
+        else asm("set.ge.u32.f16x2 %0, %1, %2;" : "=r"(ge) : "r"(word_of(v[w / 4], w % 4)), "r"(two));
+        take |= ge & (0x10001u << w);
+    }
+    return take;
+}
+// the element at a bit of reaching(), and its number in the vectors
+template <int DT, int U>
+__device__ __forceinline__ float element_of(const uint4 (&v)[U], int bit, int *e) {
+    const int w = bit & 15;
+    uint32_t word = word_of(v[0], 0);
+#pragma unroll
+    for (int i = 1; i < 4 * U; i++) word = w == i ? word_of(v[i / 4], i % 4) : word;
+    if (DT == DLLM_DTYPE_F32) {
+        *e = w;
+        return __uint_as_float(word);
+    }
+    const float2 p = pair_of<DT>(make_uint4(word, 0, 0, 0), 0);
+    *e = 2 * w + (bit >> 4);
+    return bit & 16 ? p.y : p.x;
 }
 
 template <int DT>
@@ -175,19 +248,20 @@ __device__ __noinline__ uint4 edge_vector(const unsigned char *row, const uint32
 // that holds an element at or above the threshold appends such elements to its own buffer; no
 // barrier is needed between tiles.
 //
-// Threshold: with k <= 8 j, the smallest over the 8 warps of the j-th largest of the lanes' running
-// maxima has at least k different elements at or above it.  Each warp publishes its j-th largest
-// when it meets a candidate; an old one is lower, so no order between the warps is needed.  A warp
-// whose buffer could overflow sorts it and keeps its k best: their last key is a threshold for
-// all, and what the warp meets later, with larger ids, has to be strictly above it.
+// Threshold: each warp publishes the `top` largest of its lanes' running maxima, which are different
+// elements; the k-th largest of what the 8 warps have published has k elements at or above it
+// (8 top >= 2 k, so it is close to the k-th largest of all lanes' maxima).  A warp publishes after
+// 1, 2, 3, 5, 9, ... tiles, and the first warp then passes the k-th on; older values are lower, so no
+// order between the warps is needed.  A warp whose
+// buffer could overflow sorts it and keeps its k best: their last key is a threshold for all, and
+// what the warp meets later, with larger ids, has to be strictly above it.
 template <int DT, bool MASK>
 __global__ void __launch_bounds__(BS_NT, 4) beam_chunk_kernel(dllm_beam_desc d, int chunks, ChunkSum *sums,
                                                               uint64_t *cands) {
     constexpr int VEC = Vec<DT>::N;
-    constexpr float LOG2E = 1.44269504088896340736f;
     __shared__ uint64_t buf[BS_CAP];
     __shared__ uint64_t few[BS_NT];
-    __shared__ volatile uint32_t wkey[BS_WARPS];
+    __shared__ volatile uint32_t tops[BS_NT];  // [warp][top]
     __shared__ uint32_t floor_key;
     __shared__ float wm[BS_WARPS];
     __shared__ double ws[BS_WARPS];
@@ -196,18 +270,15 @@ __global__ void __launch_bounds__(BS_NT, 4) beam_chunk_kernel(dllm_beam_desc d, 
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const int64_t row = blockIdx.x / chunks;
     const int part_no = blockIdx.x % chunks;
-    if (!beam_live(d, row)) return;
-    const int V = d.vocab, k = d.k, jth = (k + BS_WARPS - 1) / BS_WARPS;
+    const int V = d.vocab, k = d.k, top = min(32, (k + 3) / 4);
     const unsigned char *first = (const unsigned char *)d.logits + (size_t)row * d.row_stride * Vec<DT>::ESZ;
     const int shift = (int)((uintptr_t)first % 16 / Vec<DT>::ESZ);  // elements before the row in its first vector
     const uint4 *vecs = (const uint4 *)(first - shift * Vec<DT>::ESZ);
     const uint32_t *mrow = MASK ? d.mask + row * d.mask_stride : nullptr;
     const int nvec = (int)(((int64_t)V + shift + VEC - 1) / VEC), per = (nvec + chunks - 1) / chunks;
     const int v0 = per * part_no, v1 = min(v0 + per, nvec);
-
-    if (tid < BS_WARPS) wkey[tid] = 0;
-    if (tid == 0) floor_key = 0;
-    __syncthreads();
+    // vectors from here on are not wholly inside the row, or belong to the next chunk
+    const int v_full = min(v1, (int)(((int64_t)V + shift) / VEC));
 
     // Vector j; masked elements and those outside the row are -inf.  A vector that is wholly masked
     // is not read.
@@ -234,15 +305,70 @@ __global__ void __launch_bounds__(BS_NT, 4) beam_chunk_kernel(dllm_beam_desc d, 
         }
         return make_uint4(x[0], x[1], x[2], x[3]);
     };
+    uint4 next[BS_U];  // the next tile
+    auto load_tile = [&](int t0) {
+        if (!MASK && t0 + BS_U * BS_NT <= v_full && (t0 > 0 || shift == 0)) {
+#pragma unroll
+            for (int u = 0; u < BS_U; u++) next[u] = __ldg(vecs + t0 + tid + u * BS_NT);
+        } else {
+#pragma unroll
+            for (int u = 0; u < BS_U; u++) next[u] = load(t0 + u * BS_NT + tid);
+        }
+    };
+    load_tile(v0);  // under way while the beam's state is read
+    if (!beam_live(d, row)) return;
+    tops[tid] = 0;
+    if (tid == 0) floor_key = 0;
+    if (tid < BS_WARPS) wcount[tid] = 0;
+    __syncthreads();
 
     float m = -INFINITY;   // this thread's maximum so far
-    double s = 0.0;        // sum of exp(x - m)
+    double s = 0.0;        // its exponential sum, relative to sum_base(m)
     uint32_t thr = KEY_NINF + 1;   // a candidate's key has to reach it
     int count = 0;                 // candidates in this warp's buffer
     uint64_t *mine = buf + wid * BS_WCAP;
 
+    auto publish = [&] {
+        uint32_t key = okey(m);
+        for (int i = 0; i < top; i++) {
+            const uint32_t mx = __reduce_max_sync(0xffffffffu, key);
+            const uint32_t holders = __ballot_sync(0xffffffffu, key == mx);
+            if (lane == __ffs(holders) - 1) {
+                tops[wid * top + i] = mx;
+                key = 0;
+            }
+        }
+    };
+    // The k-th largest published key, without its five lowest bits: they make the keys of a lane
+    // group different, so that one comparison with each gives a key's place.
+    auto kth_published = [&] {
+        uint32_t found = 0;
+        if (k <= 16) {  // 32 keys at most
+            const uint32_t v = lane < BS_WARPS * top ? tops[lane] & ~31u | (31 - lane) : 0;
+            int above = 0;
+#pragma unroll 8
+            for (int i = 0; i < BS_WARPS * top; i++) above += (tops[i] & ~31u | (31 - i)) > v;
+            if (above == k - 1) found = v & ~31u;
+        } else {
+            for (int at = lane; at < BS_WARPS * top; at += 32) {
+                const uint32_t v = tops[at];
+                int above = 0, same = 0;
+#pragma unroll 8
+                for (int i = 0; i < BS_WARPS * top; i++) {
+                    const uint32_t o = tops[i];
+                    above += o > v;
+                    same += o == v;
+                }
+                if (above < k && above + same >= k) found = v;
+            }
+            __syncwarp();
+        }
+        // warps go on publishing meanwhile, so a lane may find none, or another one; each is a key
+        // that k elements reach
+        return __reduce_max_sync(0xffffffffu, found);
+    };
     // this warp's k best, sorted
-    auto cut = [&]() {
+    auto cut = [&] {
         for (int i = count + lane; i < BS_WCAP; i += 32) mine[i] = 0;
         __syncwarp();
         sort_desc(mine, BS_WCAP, lane, 32, [] { __syncwarp(); });
@@ -252,93 +378,110 @@ __global__ void __launch_bounds__(BS_NT, 4) beam_chunk_kernel(dllm_beam_desc d, 
             if (lane == 0) atomicMax(&floor_key, last);
             thr = max(thr, last + 1);
         }
+        if (lane == 0) wcount[wid] = count;
         __syncwarp();
     };
 
-    uint4 x[BS_U], next[BS_U];
-#pragma unroll
-    for (int u = 0; u < BS_U; u++) next[u] = load(v0 + u * BS_NT + tid);
-    bool first_tile = true;
-    for (int t0 = v0; t0 < v1; t0 += BS_NT * BS_U) {
-        float vm[BS_U];
+    // appends the elements of a tile that reach the threshold
+    auto collect = [&](const uint4 (&x)[BS_U], int t0) {
+        const uint32_t all = reaching<DT, BS_U>(x, okey_value(thr));
+        auto append = [&](uint32_t take) {
+            while (take) {
+                const int bit = __ffs(take) - 1;
+                take &= take - 1;
+                int e;  // element of this thread's tile: vector e / VEC, place e % VEC
+                const uint32_t key = okey(element_of<DT, BS_U>(x, bit, &e));
+                if (key >= thr)
+                    mine[atomicAdd(&wcount[wid], 1)] =
+                        composite(key, (t0 + e / VEC * BS_NT + tid) * VEC - shift + e % VEC);
+            }
+            __syncwarp();
+            count = *(volatile int *)&wcount[wid];
+        };
+        if (count + __reduce_add_sync(0xffffffffu, __popc(all)) <= BS_WCAP) append(all);
+        else
+#pragma unroll 1
+            for (int u = 0; u < BS_U; u++) {  // one vector of each lane at a time
+                if (count > BS_WCAP - 32 * VEC) cut();
+                append(all & (DT == DLLM_DTYPE_F32 ? 0xfu : 0xf000fu) << (4 * u));
+            }
+    };
+
+    float base = -INFINITY;  // sum_base(m), for |m| < 2^20
+    int tile = 0;
+    for (int t0 = v0; t0 < v1; t0 += BS_NT * BS_U, tile++) {
+        uint4 x[BS_U];
 #pragma unroll
         for (int u = 0; u < BS_U; u++) x[u] = next[u];
-#pragma unroll
-        for (int u = 0; u < BS_U; u++) next[u] = load(t0 + (BS_U + u) * BS_NT + tid);
-        float tm = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < BS_U; u++) {
-            vm[u] = vec_max<DT>(x[u]);
-            tm = max_keep(tm, vm[u]);
-        }
-        const float mn = max_keep(m, tm), ref = mn == -INFINITY ? 0.0f : mn;
-        float2 part = make_float2(0.0f, 0.0f);
-#pragma unroll
-        for (int u = 0; u < BS_U; u++)
-#pragma unroll
-            for (int i = 0; i < VEC / 2; i++) {
-                const float2 y = mul2(add2(pair_of<DT>(x[u], i), make_float2(-ref, -ref)), make_float2(LOG2E, LOG2E));
-                part = add2(part, make_float2(exp2_approx(y.x), exp2_approx(y.y)));
+        load_tile(t0 + BS_NT * BS_U);
+        const float tm = largest<DT, BS_U>(x);
+        Pair part(0.0f, 0.0f);
+        const Pair scale(LOG2E, LOG2E);
+        if (!__any_sync(0xffffffffu, fabsf(tm) >= BASE_EXACT || fabsf(m) >= BASE_EXACT)) {
+            if (tm > m) {
+                const float to = __fmul_rn(tm, LOG2E);
+                s *= (double)exp2_approx(__fsub_rn(base, to));
+                base = to;
+                m = tm;
             }
-        if (mn != m) s *= (double)exp2_approx((m - ref) * LOG2E);
-        m = mn;
-        s += (double)(part.x + part.y);
-
-        if (first_tile) {  // the first threshold, from every warp's first tile
-            const uint32_t kj = warp_jth(okey(m), jth);
-            if (lane == 0) wkey[wid] = kj;
-            __syncthreads();
-            first_tile = false;
-        }
-        if (__any_sync(0xffffffffu, okey(tm) >= thr)) {
-            const uint32_t kj = warp_jth(okey(m), jth);
-            if (lane == 0) wkey[wid] = kj;
-            __syncwarp();
-            uint32_t lo = wkey[0];
+            const Pair minus(-base, -base);
 #pragma unroll
-            for (int w = 1; w < BS_WARPS; w++) lo = min(lo, wkey[w]);
-            thr = max(thr, max(lo, *(volatile uint32_t *)&floor_key));
+            for (int u = 0; u < BS_U; u++)
 #pragma unroll
+                for (int i = 0; i < VEC / 2; i++) {
+                    const float2 xi = pair_of<DT>(x[u], i);
+                    part = add2(part, exp2_approx(fma2(Pair(xi.x, xi.y), scale, minus)));
+                }
+        } else {  // values from 2^20 on, or nothing above -inf yet
+            if (tm > m) {
+                s *= rebase(m, tm);
+                m = tm;
+            }
+            base = m == -INFINITY ? m : (float)sum_base(m);
+            const float ref = m == -INFINITY ? 0.0f : m, off = (float)((double)LOG2E * (double)ref - sum_base(ref));
+#pragma unroll 1
             for (int u = 0; u < BS_U; u++) {
-                if (!__any_sync(0xffffffffu, okey(vm[u]) >= thr)) continue;
-                if (count > BS_WCAP - 32 * VEC) cut();
-                const int i0 = (t0 + u * BS_NT + tid) * VEC - shift;
+                uint4 xu = x[0];
 #pragma unroll
-                for (int e = 0; e < VEC; e++) {
-                    const float2 pr = pair_of<DT>(x[u], e / 2);
-                    const float f = e & 1 ? pr.y : pr.x;
-                    const uint32_t key = okey(f);
-                    const bool take = f == f && key >= thr;
-                    const uint32_t who = __ballot_sync(0xffffffffu, take);
-                    if (take) mine[count + __popc(who & ((1u << lane) - 1))] = composite(key, i0 + e);
-                    count += __popc(who);
+                for (int w = 1; w < BS_U; w++) xu = u == w ? x[w] : xu;
+#pragma unroll
+                for (int i = 0; i < VEC / 2; i++) {
+                    const float2 xi = pair_of<DT>(xu, i);
+                    const Pair from = add2(Pair(xi.x, xi.y), Pair(-ref, -ref));
+                    part = add2(part, exp2_approx(fma2(from, scale, Pair(off, off))));
                 }
             }
         }
+        s += (double)part.sum();
+
+        if ((tile & (tile - 1)) == 0) {  // after 1, 2, 3, 5, 9, ... tiles
+            publish();
+            if (tile == 0) {  // the first threshold is taken from every warp's first tile
+                __syncthreads();
+                thr = max(thr, kth_published());
+            } else if (wid == 0) {
+                __syncwarp();
+                const uint32_t kth = kth_published();
+                if (lane == 0) atomicMax(&floor_key, kth);
+            }
+        }
+        thr = max(thr, *(volatile uint32_t *)&floor_key);
+        if (__any_sync(0xffffffffu, tm >= okey_value(thr))) collect(x, t0);
     }
 
     // the chunk's maximum and sum, and the warps' candidates that reach the last threshold
     float M = m;
 #pragma unroll
     for (int o = 16; o; o >>= 1) M = max_keep(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const uint32_t kj = warp_jth(okey(m), jth);
-    if (lane == 0) {
-        wm[wid] = M;
-        wkey[wid] = kj;
-        wcount[wid] = 0;
-    }
+    publish();
+    if (lane == 0) wm[wid] = M;
     __syncthreads();
-    uint32_t lo = wkey[0];
 #pragma unroll
-    for (int w = 0; w < BS_WARPS; w++) {
-        M = max_keep(M, wm[w]);
-        lo = min(lo, wkey[w]);
-    }
-    const float ref = M == -INFINITY ? 0.0f : M;
-    double S = m == -INFINITY ? s : s * (double)expf(m - ref);
+    for (int w = 0; w < BS_WARPS; w++) M = max_keep(M, wm[w]);
+    double S = s * rebase(m, M);
 #pragma unroll
     for (int o = 16; o; o >>= 1) S += __shfl_xor_sync(0xffffffffu, S, o);
-    const uint64_t lowest = (uint64_t)max(lo, floor_key) << 32;
+    const uint64_t lowest = (uint64_t)max(kth_published(), floor_key) << 32;
     int kept = 0;
     for (int i = lane; i < (count + 31) / 32 * 32; i += 32) {  // in place: what is kept moves towards the front
         const uint64_t c = i < count ? mine[i] : 0;
@@ -388,6 +531,11 @@ struct Best {
     int beam;
     uint64_t comp;
 };
+// Order-preserving key of a double.
+__device__ __forceinline__ uint64_t okey64(double x) {
+    const int64_t b = __double_as_longlong(x + 0.0);
+    return (uint64_t)b ^ ((uint64_t)(b >> 63) | 0x8000000000000000ull);
+}
 // whether a comes before b in the operator's order
 __device__ __forceinline__ bool before(const Best &a, const Best &b) {
     if (a.rank != b.rank) return a.rank > b.rank;
@@ -402,6 +550,7 @@ __device__ __forceinline__ bool before(const Best &a, const Best &b) {
 // reach; where that still leaves too many (equal ranks), k rounds take the best candidate that
 // comes after the one taken last.
 constexpr int BM_LEFT = 512;
+constexpr int BM_HELD = 4;  // candidates that a thread keeps in registers
 
 __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, const ChunkSum *sums,
                                                            const uint64_t *cands, int chunks) {
@@ -410,70 +559,97 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
     __shared__ int length_in[DLLM_BEAM_MAX];
     __shared__ int live[DLLM_BEAM_MAX];  // 0 nothing to offer, 1 its row's continuations, 2 ended
     __shared__ Best wbest[BS_WARPS];
-    __shared__ Best left[BM_LEFT];
+    __shared__ uint64_t left_key[BM_LEFT], left_comp[BM_LEFT];
+    __shared__ int left_beam[BM_LEFT];
     __shared__ uint32_t wkey[BS_WARPS];
     __shared__ int nleft;
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const int K = d.beams, k = d.k;
     const int64_t item = blockIdx.x;
     if (tid == 0) nleft = 0;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (int b = wid; b < K; b += BS_WARPS) {
+    // what does not come from the chunks is read while they run
+    for (int b = tid; b < K; b += BS_NT) {
         const int64_t row = item * K + b;
         const float sc = d.scores[row];
         const bool ended = d.finished && d.finished[row];
         const int len_in = d.lengths ? d.lengths[row] : 0;
-        int st = 0, kind = 0;
-        double l = 0.0;
-        if (sc != sc || sc == INFINITY) st = DLLM_ROW_ERR_NONFINITE;
-        else if (ended) kind = sc >= -FLT_MAX ? 2 : 0;
-        else if (sc >= -FLT_MAX) {
-            float M = -INFINITY;
-            for (int c = lane; c < chunks; c += 32) M = max_keep(M, sums[row * chunks + c].m);
+        const double len = fmax((double)len_in + (ended ? 0.0 : 1.0), 1.0);
+        length_in[b] = len_in;
+        score_in[b] = sc;
+        inv_len[b] = d.length_penalty != 0.0f && d.lengths ? 1.0 / pow(len, (double)d.length_penalty) : 1.0;
+        live[b] = !(sc >= -FLT_MAX && sc <= FLT_MAX) ? 0 : ended ? 2 : 1;
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int per_beam = chunks * k, N = K * per_beam;
+    const uint64_t *mine = cands + item * N;
+    // The warps take the chunks' lists in turn, so that each meets every beam's candidates: their
+    // thresholds are then alike.  Candidate number q of a warp is position q % k of its list q / k.
+    const int warp_n = ((K * chunks - wid + BS_WARPS - 1) / BS_WARPS) * k;
+    auto number = [&](int q) { return q < warp_n ? ((q / k) * BS_WARPS + wid) * k + q % k : N; };
+    uint64_t held[BM_HELD];  // this thread's first candidates
+    int at_e[BM_HELD];
 #pragma unroll
-            for (int o = 16; o; o >>= 1) M = max_keep(M, __shfl_xor_sync(0xffffffffu, M, o));
+    for (int i = 0; i < BM_HELD; i++) {
+        const int e = at_e[i] = number(lane + 32 * i);
+        held[i] = e < N && live[e / per_beam] == 1 ? mine[e] : 0;
+    }
+    for (int b = wid; b < K; b += BS_WARPS) {
+        const int64_t row = item * K + b;
+        int st = 0, kind = live[b];
+        double l = 0.0;
+        if (kind == 0 && !(score_in[b] < 0.0f)) st = DLLM_ROW_ERR_NONFINITE;  // NaN or +inf
+        if (kind == 1) {
+            float M = -INFINITY;
             double S = 0.0;
-            for (int c = lane; c < chunks; c += 32) {
-                const ChunkSum p = sums[row * chunks + c];
-                S += p.m == -INFINITY || p.m == M ? p.s : p.s * exp((double)p.m - (double)M);
+            if (chunks <= 32) {
+                const ChunkSum p = lane < chunks ? sums[row * chunks + lane] : ChunkSum{-INFINITY, 0.0f, 0.0};
+                M = p.m;
+#pragma unroll
+                for (int o = 16; o; o >>= 1) M = max_keep(M, __shfl_xor_sync(0xffffffffu, M, o));
+                S = p.s * rebase(p.m, M);
+            } else {
+                for (int c = lane; c < chunks; c += 32) M = max_keep(M, sums[row * chunks + c].m);
+#pragma unroll
+                for (int o = 16; o; o >>= 1) M = max_keep(M, __shfl_xor_sync(0xffffffffu, M, o));
+                for (int c = lane; c < chunks; c += 32) {
+                    const ChunkSum p = sums[row * chunks + c];
+                    S += p.s * rebase(p.m, M);
+                }
             }
 #pragma unroll
             for (int o = 16; o; o >>= 1) S += __shfl_xor_sync(0xffffffffu, S, o);
-            if (S != S || M == INFINITY) st = DLLM_ROW_ERR_NONFINITE;
-            else if (M > -INFINITY) {
-                kind = 1;
-                l = (double)M + log(S);
-            }
+            if (S != S || M == INFINITY) {
+                st = DLLM_ROW_ERR_NONFINITE;
+                kind = 0;
+            } else if (M > -INFINITY) l = (sum_base(M) + log2(S)) * (1.0 / (double)LOG2E);
+            else kind = 0;
         }
+        __syncwarp();
         if (lane == 0) {
-            const double len = fmax((double)len_in + (ended ? 0.0 : 1.0), 1.0);
-            length_in[b] = len_in;
-            score_in[b] = sc;
             lse[b] = l;
-            inv_len[b] = d.length_penalty != 0.0f && d.lengths ? 1.0 / pow(len, (double)d.length_penalty) : 1.0;
             live[b] = kind;
             if (d.status) d.status[row] = st;
         }
     }
     __syncthreads();
-    const int per_beam = chunks * k, N = K * per_beam;
-    const uint64_t *mine = cands + item * N;
     // candidate e: position e % k of a chunk's list; an ended beam offers its first position only
-    auto candidate = [&](int e, Best *c) {
-        const int b = e / per_beam;
-        if (live[b] == 0) return false;
+    auto candidate_of = [&](int e, int b, uint64_t comp, Best *c) {
         double cum = (double)score_in[b];
-        uint64_t comp;
+        if (live[b] == 0) return false;
         if (live[b] == 2) {
             if (e != b * per_beam) return false;
             comp = composite(0, d.eos);
         } else {
-            comp = mine[e];
             if (!comp) return false;
             cum += (double)okey_value((uint32_t)(comp >> 32)) - lse[b];
         }
         *c = {cum * inv_len[b], b, comp};
         return true;
+    };
+    auto candidate = [&](int e, Best *c) {
+        const int b = e / per_beam;
+        return candidate_of(e, b, live[b] == 1 ? mine[e] : 0, c);
     };
     auto emit = [&](int place, const Best &c, bool none) {
         float score = -INFINITY;
@@ -490,10 +666,22 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
         if (d.out_finished) d.out_finished[item * k + place] = ended || (!none && token == d.eos);
         if (d.out_lengths) d.out_lengths[item * k + place] = none ? 0 : length_in[c.beam] + (ended ? 0 : 1);
     };
-    uint32_t mx = 0;
-    for (int e = tid; e < N; e += BS_NT) {
+    auto keep = [&](int at, const Best &c) {
+        left_key[at] = okey64(c.rank);
+        left_beam[at] = c.beam;
+        left_comp[at] = c.comp;
+    };
+    uint32_t mx = 0, key[BM_HELD];
+#pragma unroll
+    for (int i = 0; i < BM_HELD; i++) {
+        const int e = at_e[i];
         Best c;
-        if (candidate(e, &c)) mx = max(mx, okey(__double2float_rd(c.rank)));
+        key[i] = e < N && candidate_of(e, e / per_beam, held[i], &c) ? okey(__double2float_rd(c.rank)) : 0;
+        mx = max(mx, key[i]);
+    }
+    for (int q = lane + 32 * BM_HELD; q < warp_n; q += 32) {
+        Best c;
+        if (candidate(number(q), &c)) mx = max(mx, okey(__double2float_rd(c.rank)));
     }
     const uint32_t kj = warp_jth(mx, (k + BS_WARPS - 1) / BS_WARPS);
     if (lane == 0) wkey[wid] = kj;
@@ -501,11 +689,18 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
     uint32_t lo = wkey[0];
 #pragma unroll
     for (int w = 1; w < BS_WARPS; w++) lo = min(lo, wkey[w]);
-    for (int e = tid; e < N; e += BS_NT) {
+#pragma unroll
+    for (int i = 0; i < BM_HELD; i++) {
+        if (key[i] == 0 || key[i] < lo) continue;
+        const int e = at_e[i], at = atomicAdd(&nleft, 1);
         Best c;
-        if (!candidate(e, &c) || okey(__double2float_rd(c.rank)) < lo) continue;
+        if (at < BM_LEFT && candidate_of(e, e / per_beam, held[i], &c)) keep(at, c);
+    }
+    for (int q = lane + 32 * BM_HELD; q < warp_n; q += 32) {
+        Best c;
+        if (!candidate(number(q), &c) || okey(__double2float_rd(c.rank)) < lo) continue;
         const int at = atomicAdd(&nleft, 1);
-        if (at < BM_LEFT) left[at] = c;
+        if (at < BM_LEFT) keep(at, c);
     }
     __syncthreads();
     int n = nleft;
@@ -535,17 +730,27 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
             Best c;
             if (!candidate(e, &c) || okey(__double2float_rd(c.rank)) < reached) continue;
             const int at = atomicAdd(&nleft, 1);
-            if (at < BM_LEFT) left[at] = c;
+            if (at < BM_LEFT) keep(at, c);
         }
         __syncthreads();
         n = nleft;
     }
     if (n <= BM_LEFT) {
         for (int i = tid; i < n; i += BS_NT) {
-            const Best c = left[i];
-            int place = 0;
-            for (int j = 0; j < n; j++) place += before(left[j], c);
-            if (place < k) emit(place, c, false);
+            const uint64_t key = left_key[i], comp = left_comp[i];
+            const int beam = left_beam[i];
+            int place = 0, same = 0;
+#pragma unroll 4
+            for (int j = 0; j < n; j++) {
+                const uint64_t other = left_key[j];
+                place += other > key;
+                same += other == key;
+            }
+            if (same > 1)
+                for (int j = 0; j < n; j++)
+                    if (left_key[j] == key)
+                        place += left_beam[j] < beam || (left_beam[j] == beam && left_comp[j] > comp);
+            if (place < k) emit(place, Best{0.0, beam, comp}, false);
         }
         for (int i = n + tid; i < k; i += BS_NT) emit(i, Best{}, true);
         return;
@@ -671,7 +876,12 @@ dllm_status launch_beam_select(const dllm_beam_desc *d, void *ws, cudaStream_t s
     uint64_t *cands = (uint64_t *)((unsigned char *)ws + ((size_t)rows * chunks * sizeof(ChunkSum) + 255) / 256 * 256);
     if (rows * chunks > INT32_MAX) return DLLM_ERR_UNSUPPORTED;
     const unsigned grid = (unsigned)(rows * chunks);
-    auto go = [&](auto kernel) { kernel<<<grid, BS_NT, 0, stream>>>(*d, chunks, sums, cands); };
+    auto go = [&](auto kernel) {
+        // room for four CTAs' buffers on an SM (the default split gave two)
+        cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                             cudaSharedmemCarveoutMaxShared);
+        kernel<<<grid, BS_NT, 0, stream>>>(*d, chunks, sums, cands);
+    };
     const bool mask = d->mask != nullptr;
     if (d->dtype == DLLM_DTYPE_F32) {
         if (mask) go(beam_chunk_kernel<DLLM_DTYPE_F32, true>);

@@ -2,11 +2,12 @@
 definition in 64 bits.
 
 Tolerance of a score.  The row's exponential sum is formed in fp32 pieces: each term has the
-exponential's relative error (2^-22) and that of its argument (three roundings of 2^-24 on
-|x - max|, whose mean under the softmax is at most log(vocab) < 13), pieces of 32 terms are added
-in fp32 (31 x 2^-24), and a rescale or two add 2^-22 each: below 4 + 39 + 31 + 8 < 96 x 2^-24 on the
-logarithm.  The score is rounded once (2^-24 of it).  Choices are exact where the ranks of the
-definition are further apart than twice that; within a beam they are always exact."""
+exponential's relative error (2^-22) and that of its argument (a rounding or three of 2^-24 on
+|x - max|, whose mean under the softmax is at most log(vocab) < 13; the constant's own rounding adds
+2^-26 of that), pieces of 32 terms are added in fp32 (31 x 2^-24), and a rescale or two add 2^-22 each:
+below 4 + 39 + 4 + 31 + 8 < 96 x 2^-24 on the logarithm.  The score is rounded once (2^-24 of it).
+Choices are exact where the ranks of the definition are further apart than twice that; within a
+beam they are always exact."""
 from __future__ import annotations
 
 import numpy as np
