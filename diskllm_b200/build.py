@@ -23,7 +23,7 @@ UNITS = [("dllm_launch.cu", []), ("dllm_capi.cu", []), ("dllm_noalloc.cu", []), 
     ("dllm_kernel_inst.cu", [f"-DDLLM_SUB={s}"]) for s in SUB_LENGTHS
 ]
 SOURCES = sorted({u[0] for u in UNITS})
-HEADERS = ["dllm_internal.h", "dllm_kernel.cuh", "dllm_chunk.cuh"]
+HEADERS = ["dllm_internal.h", "dllm_kernel.cuh", "dllm_chunk.cuh", "dllm_pair.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

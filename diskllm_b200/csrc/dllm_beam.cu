@@ -14,6 +14,7 @@
 #include <math.h>
 
 #include "dllm_internal.h"
+#include "dllm_pair.cuh"
 
 namespace dllm {
 namespace {
@@ -52,30 +53,9 @@ __device__ __forceinline__ float max_keep(float a, float b) {
     asm("max.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
-// Two fp32 values in a register pair, for the instructions that work on both.
-struct Pair {
-    unsigned long long v;
-    __device__ __forceinline__ Pair() {}
-    __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
-    __device__ __forceinline__ float sum() const {
-        float a, b;
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-        return a + b;
-    }
-};
-__device__ __forceinline__ Pair add2(Pair a, Pair b) {
-    Pair y;
-    asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(y.v) : "l"(a.v), "l"(b.v));
-    return y;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-    Pair y;
-    asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(y.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return y;
-}
 __device__ __forceinline__ Pair exp2_approx(Pair x) {
     float a, b;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v));
+    x.split(a, b);
     return Pair(exp2_approx(a), exp2_approx(b));
 }
 

@@ -12,6 +12,7 @@
 #include <math.h>
 
 #include "dllm_internal.h"
+#include "dllm_pair.cuh"
 
 namespace dllm {
 namespace {
@@ -19,7 +20,11 @@ namespace {
 // ----------------------------------------------------------------------------------------
 // rows to int8 codes
 
-constexpr int QZ_THREADS = 256;
+template <int DT>
+struct Elem {
+    static constexpr int SIZE = DT == DLLM_DTYPE_F32 ? 4 : 2;
+    static constexpr int VEC = 16 / SIZE;  // elements of 16 bytes
+};
 
 template <int DT>
 __device__ __forceinline__ float load_elem(const void *row, int64_t i) {
@@ -29,64 +34,228 @@ __device__ __forceinline__ float load_elem(const void *row, int64_t i) {
     return __half2float(__ushort_as_half(u));
 }
 
-// sum (or maximum) over the block of one double per thread
-template <bool MAX>
-__device__ __forceinline__ double block_reduce(double v, double *part) {
-    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = blockDim.x >> 5;
+template <int DT>
+__device__ __forceinline__ void unpack(const uint4 &v, float *f) {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (DT == DLLM_DTYPE_F32) f[i] = __uint_as_float(u[i]);
+        else if (DT == DLLM_DTYPE_BF16) {
+            f[2 * i] = __uint_as_float(u[i] << 16);
+            f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        } else {
+            f[2 * i] = __half2float(__ushort_as_half((unsigned short)(u[i] & 0xffffu)));
+            f[2 * i + 1] = __half2float(__ushort_as_half((unsigned short)(u[i] >> 16)));
+        }
+    }
+}
+
+// sum (or maximum) over the TPR threads of a row, in every one of them
+template <bool MAX, int TPR>
+__device__ __forceinline__ double row_reduce(double v, double *part) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         const double w = __shfl_xor_sync(0xffffffffu, v, o);
         v = MAX ? fmax(v, w) : v + w;
     }
-    if (lane == 0) part[wid] = v;
+    if (TPR == 32) return v;
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = part[0];
-    for (int i = 1; i < nw; i++) v = MAX ? fmax(v, part[i]) : v + part[i];
-    __syncthreads();
-    return v;
+    v = lane < TPR / 32 ? part[lane] : 0.0;  // sums of squares and magnitudes: zero changes neither
+#pragma unroll
+    for (int o = TPR / 64; o; o >>= 1) {
+        const double w = __shfl_xor_sync(0xffffffffu, v, o);
+        v = MAX ? fmax(v, w) : v + w;
+    }
+    return __shfl_sync(0xffffffffu, v, 0);
 }
 
-// One CTA per row.  The normalised value, the largest one and the quotient are formed in 64 bits:
-// a quotient next to a half-integer would otherwise round to the other code.
-template <int DT>
-__global__ void __launch_bounds__(QZ_THREADS) quantize_rows_kernel(const void *x, int64_t x_stride, int cols, int norm,
-                                                                   const float *w, float eps, int add_one, int8_t *q,
-                                                                   int64_t q_stride, float *scale) {
-    __shared__ double part[QZ_THREADS / 32];
-    const int tid = threadIdx.x;
-    const size_t esz = DT == DLLM_DTYPE_F32 ? 4 : 2;
-    const unsigned char *row = (const unsigned char *)x + (size_t)blockIdx.x * x_stride * esz;
-    int8_t *qrow = q + (size_t)blockIdx.x * q_stride;
+struct QuantArgs {
+    const void *x;
+    int64_t x_stride, q_stride;
+    int rows, cols, norm, add_one;
+    const float *w;
+    float eps;
+    int8_t *q;
+    float *scale;
+};
+
+// A row's scale from its largest magnitude: (float)(big / 127); 0 below the smallest normal number,
+// NaN for a row that is not finite (every product of the row is then NaN).
+__device__ __forceinline__ float scale_of(double big) {
+    if (!(big <= DBL_MAX)) return __int_as_float(0x7fc00000);
+    const float s = __double2float_rn(big / 127.0);
+    return s > FLT_MAX ? __int_as_float(0x7fc00000) : s >= FLT_MIN ? s : 0.0f;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one of them is
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// TPR threads hold a row in registers, E elements each (vectors of 16 bytes where the rows allow it).
+// A code is formed in 32 bits, x * (rs / s) * g with four roundings at most, so within
+// 127.5 * 4 * 2^-24 = 3.1e-5 of the quotient, and rounded by adding 1.5 * 2^23, whose sum holds the
+// code in its low byte; only where that lies within 6e-5 of a half-integer is it decided anew:
+//   without norm, by the sign of x - h * s for the half-integer h, which one fused operation gives exactly
+//     (a value of half the row's largest one lies there, so in 16-bit types that is no rare case);
+//   with norm, by comparing y with h * s in 64 bits, where h * s is exact.
+// With norm the sum of squares, the largest |x * g| and the scale are 64-bit too.  The factors' products
+// stay inside the range of fp32 for scales from 1e-30 to 1e30 and factors up to 1e30; rows with
+// others are divided in 64 bits.
+template <int DT, int TPR, int E, bool VECTORS, bool NORM>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quantize_rows_kernel(QuantArgs a) {
+    constexpr int VEC = VECTORS ? Elem<DT>::VEC : 1, NV = E / VEC;
+    constexpr float MAGIC = 12582912.0f;
+    __shared__ double part[2][32];
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int t = threadIdx.x % TPR, lane = threadIdx.x & 31;
+    const int64_t row = TPR < 256 ? (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR : blockIdx.x;
+    if (row >= a.rows) return;
+    const unsigned char *src = (const unsigned char *)a.x + (size_t)row * a.x_stride * Elem<DT>::SIZE;
+    int8_t *dst = a.q + (size_t)row * a.q_stride;
+    auto place = [&](int v) { return (v * TPR + t) * VEC; };  // first element of this thread's vector v
+    float x[E], g[NORM ? E : 1];
+    const float one = a.w && !a.add_one ? 0.0f : 1.0f;  // the factor is w + one
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+        const int at = place(v);
+        if (VECTORS && at + VEC <= a.cols) unpack<DT>(__ldg((const uint4 *)(src + (size_t)at * Elem<DT>::SIZE)), x + v * VEC);
+        else
+#pragma unroll
+            for (int e = 0; e < VEC; e++) x[v * VEC + e] = at + e < a.cols ? load_elem<DT>(src, at + e) : 0.0f;
+        if (NORM)
+#pragma unroll
+            for (int e = 0; e < VEC; e++) g[v * VEC + e] = a.w && at + e < a.cols ? __ldg(a.w + at + e) : 0.0f;
+    }
     double rs = 1.0;
-    if (norm) {
-        double ss = 0.0;
-        for (int i = tid; i < cols; i += QZ_THREADS) {
-            const double v = load_elem<DT>(row, i);
-            ss += v * v;
+    float s, c, gmax = 0.0f;
+    if (NORM) {
+        double ss = 0.0, big = 0.0;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            ss = fma((double)x[e], (double)x[e], ss);
+            const double y = fabs((double)x[e] * ((double)g[e] + (double)one));
+            big = y <= DBL_MAX ? fmax(big, y) : INFINITY;
+            g[e] = __fadd_rn(g[e], one);
+            gmax = fmaxf(gmax, fabsf(g[e]));
         }
-        rs = 1.0 / sqrt(block_reduce<false>(ss, part) / (double)cols + (double)eps);
+        rs = 1.0 / sqrt(row_reduce<false, TPR>(ss, part[0]) / (double)a.cols + (double)a.eps);
+        big = row_reduce<true, TPR>(big, part[1]);
+        s = rs <= DBL_MAX ? scale_of(big * rs) : __int_as_float(0x7fc00000);  // else a row of zeros and eps = 0
+        c = s > 0.0f ? __double2float_rn(rs / (double)s) : 0.0f;
+    } else {
+        float m = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; e++) m = max_nan(m, fabsf(x[e]));
+        uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(m));  // NaN is above infinity
+        if (TPR > 32) {
+            uint32_t *tops = (uint32_t *)part;
+            if (lane == 0) tops[threadIdx.x >> 5] = top;
+            __syncthreads();
+            top = __reduce_max_sync(0xffffffffu, lane < TPR / 32 ? tops[lane] : 0);
+        }
+        s = top < 0x7f800000u ? __fdiv_rn(__uint_as_float(top), 127.0f) : __int_as_float(0x7fc00000);
+        c = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
     }
-    auto value = [&](int i) {
-        double y = (double)load_elem<DT>(row, i) * rs;
-        if (w) y *= (double)w[i] + (add_one ? 1.0 : 0.0);
-        return y;
-    };
-    double big = 0.0;
-    int bad = 0;
-    for (int i = tid; i < cols; i += QZ_THREADS) {
-        const double a = fabs(value(i));
-        bad |= !(a <= DBL_MAX);
-        big = fmax(big, a);
+    if (t == 0) a.scale[row] = s;
+    const bool fast = s > 1e-30f && s < 1e30f && c > 1e-30f && c < 1e30f && gmax <= 1e30f;
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+        const int at = place(v);
+        uint32_t sum[VEC < 2 ? 2 : VEC];  // the codes are their low bytes
+        float off = 0.0f;                 // how far the quotients are from integers
+#pragma unroll
+        for (int e = 0; e < VEC; e += 2) {
+            const int i = v * VEC + e, j = VEC > 1 ? i + 1 : i;
+            Pair y = mul2(Pair(x[i], x[j]), Pair(c, c));
+            if (NORM) y = mul2(y, Pair(g[i], g[j]));
+            const Pair m = add2(y, Pair(MAGIC, MAGIC)), r = add2(m, Pair(-MAGIC, -MAGIC));
+            const Pair d = fma2(r, Pair(-1.0f, -1.0f), y);
+            float da, db, ma, mb;
+            d.split(da, db);
+            m.split(ma, mb);
+            off = fmaxf(off, fmaxf(fabsf(da), fabsf(db)));
+            sum[e] = __float_as_uint(ma);
+            sum[VEC > 1 ? e + 1 : 1] = __float_as_uint(mb);
+        }
+        if (fast && off > 0.5f - 6e-5f) {
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                const int i = v * VEC + e;
+                float about = __fmul_rn(x[i], c);
+                if (NORM) about = __fmul_rn(about, g[i]);
+                const float low = floorf(about), half = low + 0.5f;
+                if (fabsf(about - half) > 1e-4f) continue;
+                int code = (int)low;
+                if (NORM) {
+                    const double w = a.w && at + e < a.cols ? (double)__ldg(a.w + at + e) : 0.0;
+                    const double y = (double)x[i] * rs * (w + (double)one), border = (double)half * (double)s;
+                    code += y > border || (y == border && (code & 1));
+                } else {
+                    const float rest = __fmaf_rn(-half, s, x[i]);
+                    code += rest > 0.0f || (rest == 0.0f && (code & 1));
+                }
+                sum[e] = (uint32_t)code;
+            }
+        }
+        if (!fast) {  // zero rows, NaN rows, scales and factors out of range
+#pragma unroll 1
+            for (int e = 0; e < VEC; e++) {
+                if (at + e >= a.cols) break;
+                const double w = a.w ? (double)a.w[at + e] : 0.0;
+                const double y = (double)load_elem<DT>(src, at + e) * rs * (NORM ? w + (double)one : 1.0);
+                dst[at + e] = s > 0.0f ? (int8_t)__double2int_rn(y / (double)s) : 0;
+            }
+        } else if (VEC > 1 && at + VEC <= a.cols) {
+            uint32_t word[2] = {0, 0};
+#pragma unroll
+            for (int w = 0; w < VEC / 4; w++)
+                word[w] = __byte_perm(__byte_perm(sum[4 * w], sum[4 * w + 1], 0x0040),
+                                      __byte_perm(sum[4 * w + 2], sum[4 * w + 3], 0x0040), 0x5410);
+            if (VEC == 4) *(uint32_t *)(dst + at) = word[0];
+            else *(uint2 *)(dst + at) = make_uint2(word[0], word[1]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; e++)
+                if (at + e < a.cols) dst[at + e] = (int8_t)(sum[e] & 0xff);
+        }
     }
-    big = block_reduce<true>(big, part);
-    float s = __double2float_rn(big / 127.0);
-    bad = __syncthreads_or(bad | !(s <= FLT_MAX));
-    if (bad) s = __int_as_float(0x7fc00000);  // NaN: every product of the row is NaN
-    const bool zero = bad || !(s >= FLT_MIN);
-    if (!bad && zero) s = 0.0f;
-    if (tid == 0) scale[blockIdx.x] = s;
-    const double sd = (double)s;
-    for (int i = tid; i < cols; i += QZ_THREADS) qrow[i] = zero ? 0 : (int8_t)__double2int_rn(value(i) / sd);
+}
+
+// Rows too long for the registers of a CTA: read three times (from L2 after the first).
+constexpr int QZ_LONG = 1024;
+
+template <int DT>
+__global__ void __launch_bounds__(QZ_LONG) quantize_long_rows_kernel(QuantArgs a) {
+    __shared__ double part[2][32];
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int t = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    const unsigned char *src = (const unsigned char *)a.x + (size_t)row * a.x_stride * Elem<DT>::SIZE;
+    int8_t *dst = a.q + (size_t)row * a.q_stride;
+    double rs = 1.0, big = 0.0;
+    if (a.norm) {
+        double ss = 0.0;
+        for (int i = t; i < a.cols; i += QZ_LONG) {
+            const double v = load_elem<DT>(src, i);
+            ss = fma(v, v, ss);
+        }
+        rs = 1.0 / sqrt(row_reduce<false, QZ_LONG>(ss, part[0]) / (double)a.cols + (double)a.eps);
+    }
+    auto gain = [&](int i) { return a.w ? (double)a.w[i] + (a.add_one ? 1.0 : 0.0) : 1.0; };
+    for (int i = t; i < a.cols; i += QZ_LONG) {
+        const double y = fabs((double)load_elem<DT>(src, i) * gain(i));
+        big = y <= DBL_MAX ? fmax(big, y) : INFINITY;
+    }
+    big = row_reduce<true, QZ_LONG>(big, part[1]);
+    if (!(rs <= DBL_MAX)) big = INFINITY;
+    const float s = scale_of(big * rs);
+    if (t == 0) a.scale[row] = s;
+    for (int i = t; i < a.cols; i += QZ_LONG)
+        dst[i] = s > 0.0f ? (int8_t)__double2int_rn((double)load_elem<DT>(src, i) * rs * gain(i) / (double)s) : 0;
 }
 
 // ----------------------------------------------------------------------------------------
@@ -357,19 +526,45 @@ int sm_count() {
     return n;
 }
 
+// A warp per row up to 1024 columns; then a CTA, of 256 threads up to 8192 columns, and for the few
+// rows of a decode step (fewer than SMs) of 1024, whose threads have less to do one after another.
+template <int DT>
+dllm_status quantize_typed(const QuantArgs &a, cudaStream_t stream) {
+    const bool vec = (uintptr_t)a.x % 16 == 0 && (a.rows == 1 || a.x_stride * Elem<DT>::SIZE % 16 == 0);
+    auto go = [&](auto kernel, int grid, int threads) {
+        kernel<<<grid, threads, 0, stream>>>(a);
+        return cudaGetLastError() == cudaSuccess ? DLLM_OK : DLLM_ERR_CUDA;
+    };
+#define DLLM_QUANTIZE(TPR, E, GRID)                                                            \
+    do {                                                                                       \
+        const int threads = TPR < 256 ? 256 : TPR;                                             \
+        if (a.norm) return vec ? go(quantize_rows_kernel<DT, TPR, E, true, true>, GRID, threads)  \
+                               : go(quantize_rows_kernel<DT, TPR, E, false, true>, GRID, threads); \
+        return vec ? go(quantize_rows_kernel<DT, TPR, E, true, false>, GRID, threads)          \
+                   : go(quantize_rows_kernel<DT, TPR, E, false, false>, GRID, threads);        \
+    } while (0)
+    const int groups = (a.rows + 7) / 8;
+    const bool many = a.rows >= 148;
+    if (a.cols <= 512) DLLM_QUANTIZE(32, 16, groups);
+    if (a.cols <= 1024 && many) DLLM_QUANTIZE(32, 32, groups);
+    if (a.cols <= 4096 && many) DLLM_QUANTIZE(256, 16, a.rows);
+    if (a.cols <= 8192 && many) DLLM_QUANTIZE(256, 32, a.rows);
+    if (a.cols <= 8192) DLLM_QUANTIZE(1024, 8, a.rows);
+    if (a.cols <= 16384) DLLM_QUANTIZE(1024, 16, a.rows);
+#undef DLLM_QUANTIZE
+    return go(quantize_long_rows_kernel<DT>, a.rows, QZ_LONG);
+}
+
 }  // namespace
 
 dllm_status launch_quantize_i8(int rows, int cols, const void *x, int64_t x_stride, int x_dtype, int norm,
                                const float *norm_w, float eps, int add_one, int8_t *q, int64_t q_stride, float *scale,
                                cudaStream_t stream) {
     if (rows == 0) return DLLM_OK;
-    auto go = [&](auto kernel) {
-        kernel<<<rows, QZ_THREADS, 0, stream>>>(x, x_stride, cols, norm, norm_w, eps, add_one, q, q_stride, scale);
-        return cudaGetLastError() == cudaSuccess ? DLLM_OK : DLLM_ERR_CUDA;
-    };
-    if (x_dtype == DLLM_DTYPE_F32) return go(quantize_rows_kernel<DLLM_DTYPE_F32>);
-    if (x_dtype == DLLM_DTYPE_BF16) return go(quantize_rows_kernel<DLLM_DTYPE_BF16>);
-    return go(quantize_rows_kernel<DLLM_DTYPE_F16>);
+    const QuantArgs a = {x, x_stride, q_stride, rows, cols, norm, add_one, norm_w, eps, q, scale};
+    if (x_dtype == DLLM_DTYPE_F32) return quantize_typed<DLLM_DTYPE_F32>(a, stream);
+    if (x_dtype == DLLM_DTYPE_BF16) return quantize_typed<DLLM_DTYPE_BF16>(a, stream);
+    return quantize_typed<DLLM_DTYPE_F16>(a, stream);
 }
 
 dllm_status launch_matmul_i8(int m, int n, int k, const int8_t *a, int64_t lda, const float *sa, const int8_t *b,
