@@ -300,9 +300,9 @@ static dllm_status check_matmul_i8(int m, int n, int k, float softcap) {
 
 static dllm_status run_matmul_i8(int m, int n, int k, const int8_t *a, int64_t lda, const float *sa, const int8_t *b,
                                  int64_t ldb, const float *sb, float softcap, void *out, int64_t ldo, int out_dtype,
-                                 int32_t *status, cudaStream_t stream) {
+                                 int32_t *status, bool early_b, cudaStream_t stream) {
     const dllm_status st = launch_matmul_i8(m, n, k, a, lda, sa, b, ldb, sb, softcap, out, ldo, out_dtype, status,
-                                            stream);
+                                            early_b, stream);
     if (st == DLLM_ERR_CUDA) set_error("int8 product kernel launch", cudaGetLastError());
     return st;
 }
@@ -321,7 +321,7 @@ extern "C" dllm_status dllm_cuda_matmul_i8(int m, int n, int k, const int8_t *a,
     if (out_stride < n) return invalid("out_stride < n");
     if ((uintptr_t)out % dtype_bytes(out_dtype) != 0) return invalid("out is not aligned to its type");
     return run_matmul_i8(m, n, k, a, a_stride, a_scale, b, b_stride, b_scale, softcap, out, out_stride, out_dtype,
-                         status, (cudaStream_t)stream);
+                         status, false, (cudaStream_t)stream);
 }
 
 static int64_t code_stride(int cols) { return ((int64_t)cols + 15) / 16 * 16; }
@@ -351,8 +351,9 @@ extern "C" dllm_status dllm_cuda_lmhead_logits_i8(int rows, int hidden, int voca
     st = dllm_cuda_quantize_rows_i8(rows, hidden, h, hidden, DLLM_DTYPE_F32, 1, norm_w, eps, add_one, q,
                                     code_stride(hidden), scale, stream);
     if (st != DLLM_OK) return st;
+    // the product starts while the codes are made: only they, not the weights, come from the kernel before it
     return run_matmul_i8(rows, vocab, hidden, q, code_stride(hidden), scale, w, w_stride, w_scale, softcap, logits,
-                         vocab, DLLM_DTYPE_F32, status, (cudaStream_t)stream);
+                         vocab, DLLM_DTYPE_F32, status, true, (cudaStream_t)stream);
 }
 
 // ----------------------------------------------------------------------------------------

@@ -106,13 +106,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one of t
 // stay inside the range of fp32 for scales from 1e-30 to 1e30 and factors up to 1e30; rows with
 // others are divided in 64 bits.
 template <int DT, int TPR, int E, bool VECTORS, bool NORM>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quantize_rows_kernel(QuantArgs a) {
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) quantize_rows_kernel(QuantArgs a) {
     constexpr int VEC = VECTORS ? Elem<DT>::VEC : 1, NV = E / VEC;
     constexpr float MAGIC = 12582912.0f;
     __shared__ double part[2][32];
     asm volatile("griddepcontrol.launch_dependents;");
     const int t = threadIdx.x % TPR, lane = threadIdx.x & 31;
-    const int64_t row = TPR < 256 ? (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR : blockIdx.x;
+    const int64_t row = TPR == 32 ? (int64_t)blockIdx.x * 8 + threadIdx.x / 32 : blockIdx.x;
     if (row >= a.rows) return;
     const unsigned char *src = (const unsigned char *)a.x + (size_t)row * a.x_stride * Elem<DT>::SIZE;
     int8_t *dst = a.q + (size_t)row * a.q_stride;
@@ -277,7 +277,7 @@ constexpr int MM_KB = 128;                   // bytes of k in a pipeline stage (
 constexpr int MM_EPI_WARPS = 8;
 constexpr int MM_THREADS = 64 + 32 * MM_EPI_WARPS;
 constexpr int MM_MAX_STAGES = 12;
-constexpr int MM_SMEM = 220 * 1024;          // stages, with 1 KB to align them
+constexpr int MM_SMEM = 216 * 1024;          // stages, with 1 KB to align them
 
 struct MmArgs {
     const float *sa, *sb;
@@ -289,6 +289,7 @@ struct MmArgs {
     int token_tiles;
     int stages;
     int tmem_cols;   // allocated columns: two accumulators
+    int early_b;     // a and its scales come from the kernel before, which may still run; b does not
     float softcap;
 };
 
@@ -363,6 +364,28 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, int (&r)[16]) {
         : "memory");
 }
 
+// tanh of both values.  Up to 1: z * (1 + z^2 Q(z^2)), Q of degree 6 fitted to tanh(z) / z by reweighted
+// least squares on Chebyshev points (relative error 5e-9; evaluated in fp32, 1.8 x 2^-24).  Above:
+// 1 - 2 / (e^2z + 1), whose error there is under 4 x 2^-24, for the warps that hold such a value.
+__device__ __forceinline__ Pair tanh2(Pair z) {
+    const Pair u = mul2(z, z);
+    Pair q(-3.584515071e-04f, -3.584515071e-04f);
+    q = fma2(q, u, Pair(2.301362809e-03f, 2.301362809e-03f));
+    q = fma2(q, u, Pair(-7.946103811e-03f, -7.946103811e-03f));
+    q = fma2(q, u, Pair(2.148665674e-02f, 2.148665674e-02f));
+    q = fma2(q, u, Pair(-5.387980118e-02f, -5.387980118e-02f));
+    q = fma2(q, u, Pair(1.333234459e-01f, 1.333234459e-01f));
+    q = fma2(q, u, Pair(-3.333329558e-01f, -3.333329558e-01f));
+    q = fma2(q, u, Pair(1.0f, 1.0f));
+    return mul2(q, z);
+}
+__device__ __forceinline__ float tanh_above_one(float z) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(fabsf(z), 2.88539008177792681f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(e, 1.0f)));
+    return copysignf(__fmaf_rn(-2.0f, r, 1.0f), z);
+}
+
 // Persistent, one CTA per SM.  Warp 0 copies tiles (TMA), warp 1 issues the products, warps 2 to 9
 // scale and store; two accumulators, so that a tile's stores run under the next tile's products.
 template <int DT, bool CAP>
@@ -370,6 +393,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_kernel(const __grid_c
                                                                   const __grid_constant__ CUtensorMap map_b, MmArgs p) {
     extern __shared__ unsigned char raw[];
     __shared__ __align__(8) uint64_t bars[2 * MM_MAX_STAGES + 5];
+    __shared__ __align__(16) float scales[MM_EPI_WARPS][256];  // a warp's copy of its tile's token scales
     __shared__ uint32_t tmem_base;
     __shared__ int gave_up;
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
@@ -406,18 +430,47 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_kernel(const __grid_c
 
     if (wid == 0) {
         if (lane == 0) {
-            uint32_t step = 0;  // k blocks so far: stage step % stages, use step / stages
-            bool ok = true;
-            for (int64_t t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
-                const int y_b = (int)(t / p.token_tiles) * MM_ROWS, y_a = (int)(t % p.token_tiles) * p.nt;
-                for (int kb = 0; kb < kblocks; kb++, step++) {
-                    const uint32_t s = step % p.stages, use = step / p.stages;
-                    if (use > 0 && !(ok = mbar_wait(empty + 8 * s, (use - 1) & 1, &gave_up))) break;
-                    const uint32_t at = tiles + s * stage_bytes, bar = full + 8 * s;
-                    mbar_expect(bar, stage_bytes);
-                    tma_load(at, &map_b, kb * MM_KB, y_b, bar);
-                    tma_load(at + MM_ROWS * MM_KB, &map_a, kb * MM_KB, y_a, bar);
+            uint32_t step;  // k blocks so far: stage step % stages, use step / stages
+            int64_t t;
+            int kb, y_a, y_b;  // k block, and the tile's first token and channel
+            uint32_t s;        // step % stages
+            auto tile = [&] {
+                y_b = (int)(t / p.token_tiles) * MM_ROWS;
+                y_a = (int)(t % p.token_tiles) * p.nt;
+            };
+            auto begin = [&] {
+                t = blockIdx.x;
+                kb = 0;
+                s = step = 0;
+                tile();
+            };
+            auto advance = [&] {
+                step++;
+                if (++s == (uint32_t)p.stages) s = 0;
+                if (++kb == kblocks) {
+                    kb = 0;
+                    t += gridDim.x;
+                    tile();
                 }
+            };
+            auto load_b = [&] {
+                mbar_expect(full + 8 * s, stage_bytes);
+                tma_load(tiles + s * stage_bytes, &map_b, kb * MM_KB, y_b, full + 8 * s);
+            };
+            auto load_a = [&] {
+                tma_load(tiles + s * stage_bytes + MM_ROWS * MM_KB, &map_a, kb * MM_KB, y_a, full + 8 * s);
+            };
+            begin();
+            if (p.early_b) {  // fill the pipeline with b while a is still being made
+                for (; step < (uint32_t)p.stages && t < ntiles; advance()) load_b();
+                const uint32_t filled = step;
+                asm volatile("griddepcontrol.wait;" ::: "memory");
+                for (begin(); step < filled; advance()) load_a();
+            }
+            for (; t < ntiles; advance()) {
+                if (step >= (uint32_t)p.stages && !mbar_wait(empty + 8 * s, (step / p.stages - 1) & 1, &gave_up)) break;
+                load_b();
+                load_a();
             }
             // no copy may be in flight when the CTA ends, also where a wait ran out
             volatile int alone = 0;
@@ -455,28 +508,65 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_kernel(const __grid_c
         __syncwarp();
     } else {
         const int quarter = wid & 3, half = (wid - 2) >> 2;  // tensor memory lanes of a warp: 32 * (warp % 4)
+        float *sa = scales[wid - 2];
+        if (p.early_b) asm volatile("griddepcontrol.wait;" ::: "memory");
         uint32_t it = 0;
         for (int64_t t = blockIdx.x; t < ntiles; t += gridDim.x, it++) {
             const uint32_t acc = it & 1;
             const int ch = (int)(t / p.token_tiles) * MM_ROWS + quarter * 32 + lane;
             const int t0 = (int)(t % p.token_tiles) * p.nt;
-            const float sb = ch < p.n ? __ldg(p.sb + ch) : 0.0f;
+            float sb = ch < p.n ? __ldg(p.sb + ch) : 0.0f;
+            if (CAP) sb = __fdiv_rn(sb, p.softcap);
+            if (it == 0 || p.token_tiles > 1) {
+                __syncwarp();
+                for (int i = lane; i < p.nt; i += 32) sa[i] = t0 + i < p.m ? __ldg(p.sa + t0 + i) : 0.0f;
+                __syncwarp();
+            }
             int ok = mbar_wait(done + 8 * acc, (it >> 1) & 1, &gave_up);
             if (!__all_sync(0xffffffffu, ok)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             for (int c = half * 16; c < p.nt; c += 32) {
                 int r[16];
                 tmem_load16(tmem + acc * p.nt + c + ((uint32_t)quarter << 21), r);
-                if (ch < p.n) {
+                float v[16];
+                float big = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        const int token = t0 + c + j;
-                        if (token < p.m) {
-                            float v = __fmul_rn(__fmul_rn((float)r[j], __ldg(p.sa + token)), sb);
-                            if (CAP) v = __fmul_rn(p.softcap, tanhf(__fdiv_rn(v, p.softcap)));
-                            store_out<DT>(p.out, token * p.ldo + ch, v);
+                for (int j = 0; j < 16; j += 4) {
+                    const float4 s4 = *(const float4 *)(sa + c + j);
+                    Pair lo = mul2(mul2(Pair((float)r[j], (float)r[j + 1]), Pair(s4.x, s4.y)), Pair(sb, sb));
+                    Pair hi = mul2(mul2(Pair((float)r[j + 2], (float)r[j + 3]), Pair(s4.z, s4.w)), Pair(sb, sb));
+                    if (CAP) {
+                        float z[4];
+                        lo.split(z[0], z[1]);
+                        hi.split(z[2], z[3]);
+                        lo = tanh2(lo);
+                        hi = tanh2(hi);
+                        big = fmaxf(fmaxf(fabsf(z[0]), fabsf(z[1])), fmaxf(fabsf(z[2]), fabsf(z[3])));
+                        if (__any_sync(0xffffffffu, big > 1.0f)) {
+                            float y[4];
+                            lo.split(y[0], y[1]);
+                            hi.split(y[2], y[3]);
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                if (fabsf(z[i]) > 1.0f) y[i] = tanh_above_one(z[i]);
+                            lo = Pair(y[0], y[1]);
+                            hi = Pair(y[2], y[3]);
                         }
+                        lo = mul2(lo, Pair(p.softcap, p.softcap));
+                        hi = mul2(hi, Pair(p.softcap, p.softcap));
                     }
+                    lo.split(v[j], v[j + 1]);
+                    hi.split(v[j + 2], v[j + 3]);
+                }
+                if (ch >= p.n) continue;
+                int64_t at = (int64_t)(t0 + c) * p.ldo + ch;
+                if (t0 + c + 16 <= p.m) {
+#pragma unroll
+                    for (int j = 0; j < 16; j++, at += p.ldo) store_out<DT>(p.out, at, v[j]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; j++, at += p.ldo)
+                        if (t0 + c + j < p.m) store_out<DT>(p.out, at, v[j]);
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -537,7 +627,7 @@ dllm_status quantize_typed(const QuantArgs &a, cudaStream_t stream) {
     };
 #define DLLM_QUANTIZE(TPR, E, GRID)                                                            \
     do {                                                                                       \
-        const int threads = TPR < 256 ? 256 : TPR;                                             \
+        const int threads = TPR == 32 ? 256 : TPR;                                             \
         if (a.norm) return vec ? go(quantize_rows_kernel<DT, TPR, E, true, true>, GRID, threads)  \
                                : go(quantize_rows_kernel<DT, TPR, E, false, true>, GRID, threads); \
         return vec ? go(quantize_rows_kernel<DT, TPR, E, true, false>, GRID, threads)          \
@@ -547,7 +637,8 @@ dllm_status quantize_typed(const QuantArgs &a, cudaStream_t stream) {
     const bool many = a.rows >= 148;
     if (a.cols <= 512) DLLM_QUANTIZE(32, 16, groups);
     if (a.cols <= 1024 && many) DLLM_QUANTIZE(32, 32, groups);
-    if (a.cols <= 4096 && many) DLLM_QUANTIZE(256, 16, a.rows);
+    if (a.cols <= 2048 && many) DLLM_QUANTIZE(128, 16, a.rows);
+    if (a.cols <= 4096 && many) DLLM_QUANTIZE(128, 32, a.rows);
     if (a.cols <= 8192 && many) DLLM_QUANTIZE(256, 32, a.rows);
     if (a.cols <= 8192) DLLM_QUANTIZE(1024, 8, a.rows);
     if (a.cols <= 16384) DLLM_QUANTIZE(1024, 16, a.rows);
@@ -569,7 +660,7 @@ dllm_status launch_quantize_i8(int rows, int cols, const void *x, int64_t x_stri
 
 dllm_status launch_matmul_i8(int m, int n, int k, const int8_t *a, int64_t lda, const float *sa, const int8_t *b,
                              int64_t ldb, const float *sb, float softcap, void *out, int64_t ldo, int out_dtype,
-                             int32_t *status, cudaStream_t stream) {
+                             int32_t *status, bool early_b, cudaStream_t stream) {
     if (m == 0 || n == 0) return DLLM_OK;
     MmArgs p = {};
     p.sa = sa;
@@ -581,6 +672,7 @@ dllm_status launch_matmul_i8(int m, int n, int k, const int8_t *a, int64_t lda, 
     p.n = n;
     p.k = k;
     p.softcap = softcap;
+    p.early_b = early_b;
     // token tiles of equal size, at most 256 (the widest instruction)
     p.token_tiles = (m + 255) / 256;
     p.nt = ((m + p.token_tiles - 1) / p.token_tiles + 15) / 16 * 16;
@@ -595,8 +687,18 @@ dllm_status launch_matmul_i8(int m, int n, int k, const int8_t *a, int64_t lda, 
     auto go = [&](auto kernel) {
         if (cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MM_SMEM) != cudaSuccess)
             return DLLM_ERR_CUDA;
-        kernel<<<grid, MM_THREADS, MM_SMEM, stream>>>(map_a, map_b, p);
-        return cudaGetLastError() == cudaSuccess ? DLLM_OK : DLLM_ERR_CUDA;
+        // with early_b, launched while the kernel that makes a runs; it waits for it on the GPU
+        cudaLaunchAttribute attr = {};
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(grid);
+        cfg.blockDim = dim3(MM_THREADS);
+        cfg.dynamicSmemBytes = MM_SMEM;
+        cfg.stream = stream;
+        cfg.attrs = &attr;
+        cfg.numAttrs = early_b ? 1 : 0;
+        return cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, p) == cudaSuccess ? DLLM_OK : DLLM_ERR_CUDA;
     };
     const bool cap = softcap > 0.0f;
     if (out_dtype == DLLM_DTYPE_F32)

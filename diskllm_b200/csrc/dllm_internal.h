@@ -124,7 +124,7 @@ dllm_status launch_quantize_i8(int rows, int cols, const void *x, int64_t x_stri
                                cudaStream_t stream);
 dllm_status launch_matmul_i8(int m, int n, int k, const int8_t *a, int64_t lda, const float *sa, const int8_t *b,
                              int64_t ldb, const float *sb, float softcap, void *out, int64_t ldo, int out_dtype,
-                             int32_t *status, cudaStream_t stream);
+                             int32_t *status, bool early_b, cudaStream_t stream);
 size_t beam_ws_bytes(const dllm_beam_desc *d);
 dllm_status launch_beam_select(const dllm_beam_desc *d, void *ws, cudaStream_t stream);
 dllm_status launch_beam_reorder(int batch, int beams, const int32_t *parent, int ntensors, void *const *tensors,
