@@ -583,6 +583,149 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_kernel(const __grid_c
     }
 }
 
+// The same product for few tiles: a cluster of CTAs per tile, each taking a part of k.  The parts'
+// integer sums are exchanged through distributed shared memory (over the drained pipeline stages):
+// every CTA adds up and stores 128 / cluster of the tile's channels.
+template <int DT, bool CAP>
+__global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_split_kernel(const __grid_constant__ CUtensorMap map_a,
+                                                                        const __grid_constant__ CUtensorMap map_b,
+                                                                        MmArgs p) {
+    extern __shared__ unsigned char raw[];
+    __shared__ __align__(8) uint64_t bars[2 * MM_MAX_STAGES + 1];
+    __shared__ uint32_t tmem_base;
+    __shared__ int gave_up;
+    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+    uint32_t rank, parts;
+    asm("mov.u32 %0, %cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %cluster_nctarank;" : "=r"(parts));
+    const uint32_t pad = (1024 - (smem_addr(raw) & 1023)) & 1023, tiles = smem_addr(raw) + pad;
+    const int stage_bytes = (MM_ROWS + p.nt) * MM_KB;
+    const uint32_t full = smem_addr(bars), empty = full + 8 * MM_MAX_STAGES, done = full + 16 * MM_MAX_STAGES;
+    const int kblocks = (p.k + MM_KB - 1) / MM_KB;
+    const int k0 = (int)((int64_t)kblocks * rank / parts), n = (int)((int64_t)kblocks * (rank + 1) / parts) - k0;
+    const int t = blockIdx.x / parts, y_b = t / p.token_tiles * MM_ROWS, y_a = t % p.token_tiles * p.nt;
+
+    if (wid == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
+                     "r"(p.tmem_cols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if (tid == 0) {
+        for (int i = 0; i < p.stages; i++) {
+            mbar_init(full + 8 * i, 1);
+            mbar_init(empty + 8 * i, 1);
+        }
+        mbar_init(done, 1);
+        gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = tmem_base;
+
+    if (wid == 0) {
+        if (lane == 0) {
+            auto load_b = [&](int i) {
+                const uint32_t s = i % p.stages;
+                mbar_expect(full + 8 * s, stage_bytes);
+                tma_load(tiles + s * stage_bytes, &map_b, (k0 + i) * MM_KB, y_b, full + 8 * s);
+            };
+            auto load_a = [&](int i) {
+                const uint32_t s = i % p.stages;
+                tma_load(tiles + s * stage_bytes + MM_ROWS * MM_KB, &map_a, (k0 + i) * MM_KB, y_a, full + 8 * s);
+            };
+            const int first = n < p.stages ? n : p.stages;
+            int i = 0;
+            for (; i < first; i++) load_b(i);
+            if (p.early_b) asm volatile("griddepcontrol.wait;" ::: "memory");
+            for (i = 0; i < first; i++) load_a(i);
+            for (; i < n; i++) {
+                if (!mbar_wait(empty + 8 * (i % p.stages), (i / p.stages - 1) & 1, &gave_up)) break;
+                load_b(i);
+                load_a(i);
+            }
+            volatile int alone = 0;
+            for (int j = i < p.stages ? 0 : i - p.stages; j < i; j++)
+                mbar_wait(full + 8 * (j % p.stages), (j / p.stages) & 1, &alone);
+        }
+        __syncwarp();
+    } else if (wid == 1) {
+        if (lane == 0) {
+            const uint32_t idesc = 2u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(p.nt >> 3) << 17 | (MM_ROWS >> 4) << 24;
+            for (int i = 0; i < n; i++) {
+                const uint32_t s = i % p.stages;
+                if (!mbar_wait(full + 8 * s, (i / p.stages) & 1, &gave_up)) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t da = operand_desc(tiles + s * stage_bytes),
+                               db = operand_desc(tiles + s * stage_bytes + MM_ROWS * MM_KB);
+#pragma unroll
+                for (int j = 0; j < MM_KB / 32; j++) mma_i8(tmem, da + 2 * j, db + 2 * j, idesc, i > 0 || j > 0);
+                mma_commit(empty + 8 * s);
+            }
+            mma_commit(done);
+        }
+        __syncwarp();
+    }
+    // every thread: this CTA's products are complete (bounded), then every CTA's, so that all stages are free
+    volatile int alone = 0;
+    if (!mbar_wait(done, 0, &alone)) gave_up = 1;
+    __syncwarp();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    // channel c of the tile belongs to rank c / own; its sums lie there as [part][token][own]
+    const int own = MM_ROWS / (int)parts;
+    if (wid >= 2) {
+        const int quarter = wid & 3, half = (wid - 2) >> 2, c = quarter * 32 + lane;
+        uint32_t there;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(tiles), "r"((uint32_t)(c / own)));
+        there += (rank * p.nt * own + c % own) * 4;
+        for (int col = half * 16; col < p.nt; col += 32) {
+            int r[16];
+            tmem_load16(tmem + col + ((uint32_t)quarter << 21), r);
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there + (col + j) * own * 4), "r"(r[j]) : "memory");
+        }
+        __syncwarp();
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (wid == 1) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols));
+        if (lane == 0 && gave_up && p.status) atomicOr(p.status, DLLM_ROW_ERR_TIMEOUT);
+    }
+    if (p.early_b) asm volatile("griddepcontrol.wait;" ::: "memory");  // the token scales
+    const int *sums = (const int *)(raw + pad);
+    for (int i = tid; i < own * p.nt / 2; i += MM_THREADS) {  // two tokens of a channel
+        const int c = i % own, col = i / own * 2, ch = y_b + (int)rank * own + c, token = y_a + col;
+        if (ch >= p.n || token >= p.m) continue;
+        int a0 = 0, a1 = 0;
+        for (int q = 0; q < (int)parts; q++) {
+            a0 += sums[(q * p.nt + col) * own + c];
+            a1 += sums[(q * p.nt + col + 1) * own + c];
+        }
+        float sb = __ldg(p.sb + ch), v0, v1;
+        if (CAP) sb = __fdiv_rn(sb, p.softcap);
+        const bool two = token + 1 < p.m;
+        Pair v = mul2(mul2(Pair((float)a0, (float)a1), Pair(__ldg(p.sa + token), two ? __ldg(p.sa + token + 1) : 0.0f)),
+                      Pair(sb, sb));
+        if (CAP) {
+            float z0, z1;
+            v.split(z0, z1);
+            tanh2(v).split(v0, v1);
+            if (fabsf(z0) > 1.0f) v0 = tanh_above_one(z0);
+            if (fabsf(z1) > 1.0f) v1 = tanh_above_one(z1);
+            v = mul2(Pair(v0, v1), Pair(p.softcap, p.softcap));
+        }
+        v.split(v0, v1);
+        store_out<DT>(p.out, (int64_t)token * p.ldo + ch, v0);
+        if (two) store_out<DT>(p.out, (int64_t)(token + 1) * p.ldo + ch, v1);
+    }
+}
+
 using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -683,29 +826,38 @@ dllm_status launch_matmul_i8(int m, int n, int k, const int8_t *a, int64_t lda, 
     CUtensorMap map_a, map_b;
     if (!code_map(&map_a, a, m, k, lda, p.nt) || !code_map(&map_b, b, n, k, ldb, MM_ROWS)) return DLLM_ERR_CUDA;
     const int64_t tiles = (int64_t)((n + MM_ROWS - 1) / MM_ROWS) * p.token_tiles;
-    const int sms = sm_count(), grid = tiles < sms ? (int)tiles : sms;
+    const int sms = sm_count(), kblocks = (k + MM_KB - 1) / MM_KB;
+    // few tiles: split k over a cluster of up to 8 CTAs, while the SMs suffice and a part has 4 blocks
+    int parts = 1;
+    while (parts < 8 && tiles * parts * 2 <= sms && kblocks >= parts * 8) parts *= 2;
     auto go = [&](auto kernel) {
         if (cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MM_SMEM) != cudaSuccess)
             return DLLM_ERR_CUDA;
-        // with early_b, launched while the kernel that makes a runs; it waits for it on the GPU
-        cudaLaunchAttribute attr = {};
-        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr.val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchAttribute attr[2] = {};
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(grid);
+        cfg.gridDim = dim3(parts > 1 ? (unsigned)(tiles * parts) : (unsigned)(tiles < sms ? tiles : sms));
         cfg.blockDim = dim3(MM_THREADS);
         cfg.dynamicSmemBytes = MM_SMEM;
         cfg.stream = stream;
-        cfg.attrs = &attr;
-        cfg.numAttrs = early_b ? 1 : 0;
+        cfg.attrs = attr;
+        if (early_b) {  // launched while the kernel that makes a runs; it waits for it on the GPU
+            attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+        }
+        if (parts > 1) {
+            attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+            attr[cfg.numAttrs++].val.clusterDim = {(unsigned)parts, 1, 1};
+        }
         return cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, p) == cudaSuccess ? DLLM_OK : DLLM_ERR_CUDA;
     };
     const bool cap = softcap > 0.0f;
-    if (out_dtype == DLLM_DTYPE_F32)
-        return cap ? go(matmul_i8_kernel<DLLM_DTYPE_F32, true>) : go(matmul_i8_kernel<DLLM_DTYPE_F32, false>);
-    if (out_dtype == DLLM_DTYPE_BF16)
-        return cap ? go(matmul_i8_kernel<DLLM_DTYPE_BF16, true>) : go(matmul_i8_kernel<DLLM_DTYPE_BF16, false>);
-    return cap ? go(matmul_i8_kernel<DLLM_DTYPE_F16, true>) : go(matmul_i8_kernel<DLLM_DTYPE_F16, false>);
+#define DLLM_MATMUL(DT)                                                                                   \
+    (parts > 1 ? (cap ? go(matmul_i8_split_kernel<DT, true>) : go(matmul_i8_split_kernel<DT, false>))     \
+               : (cap ? go(matmul_i8_kernel<DT, true>) : go(matmul_i8_kernel<DT, false>)))
+    if (out_dtype == DLLM_DTYPE_F32) return DLLM_MATMUL(DLLM_DTYPE_F32);
+    if (out_dtype == DLLM_DTYPE_BF16) return DLLM_MATMUL(DLLM_DTYPE_BF16);
+    return DLLM_MATMUL(DLLM_DTYPE_F16);
+#undef DLLM_MATMUL
 }
 
 }  // namespace dllm
