@@ -843,6 +843,14 @@ __global__ void __launch_bounds__(RO_NT) beam_reorder_kernel(ReorderArgs a) {
 
 }  // namespace
 
+template <auto Kernel>
+static void launch_chunks(unsigned grid, const dllm_beam_desc &d, int chunks, ChunkSum *sums, uint64_t *cands,
+                          cudaStream_t stream) {
+    // room for four CTAs' buffers on an SM
+    set_once<Kernel>(cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    Kernel<<<grid, BS_NT, 0, stream>>>(d, chunks, sums, cands);
+}
+
 size_t beam_ws_bytes(const dllm_beam_desc *d) {
     const int64_t rows = (int64_t)d->batch * d->beams;
     const size_t n = (size_t)rows * beam_chunks(rows, d->vocab, d->dtype);
@@ -856,23 +864,13 @@ dllm_status launch_beam_select(const dllm_beam_desc *d, void *ws, cudaStream_t s
     uint64_t *cands = (uint64_t *)((unsigned char *)ws + ((size_t)rows * chunks * sizeof(ChunkSum) + 255) / 256 * 256);
     if (rows * chunks > INT32_MAX) return DLLM_ERR_UNSUPPORTED;
     const unsigned grid = (unsigned)(rows * chunks);
-    auto go = [&](auto kernel) {
-        // room for four CTAs' buffers on an SM (the default split gave two)
-        cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
-                             cudaSharedmemCarveoutMaxShared);
-        kernel<<<grid, BS_NT, 0, stream>>>(*d, chunks, sums, cands);
-    };
-    const bool mask = d->mask != nullptr;
-    if (d->dtype == DLLM_DTYPE_F32) {
-        if (mask) go(beam_chunk_kernel<DLLM_DTYPE_F32, true>);
-        else go(beam_chunk_kernel<DLLM_DTYPE_F32, false>);
-    } else if (d->dtype == DLLM_DTYPE_BF16) {
-        if (mask) go(beam_chunk_kernel<DLLM_DTYPE_BF16, true>);
-        else go(beam_chunk_kernel<DLLM_DTYPE_BF16, false>);
-    } else {
-        if (mask) go(beam_chunk_kernel<DLLM_DTYPE_F16, true>);
-        else go(beam_chunk_kernel<DLLM_DTYPE_F16, false>);
-    }
+#define DLLM_CHUNKS(DT)                                                                                \
+    (d->mask ? launch_chunks<beam_chunk_kernel<DT, true>>(grid, *d, chunks, sums, cands, stream)       \
+             : launch_chunks<beam_chunk_kernel<DT, false>>(grid, *d, chunks, sums, cands, stream))
+    if (d->dtype == DLLM_DTYPE_F32) DLLM_CHUNKS(DLLM_DTYPE_F32);
+    else if (d->dtype == DLLM_DTYPE_BF16) DLLM_CHUNKS(DLLM_DTYPE_BF16);
+    else DLLM_CHUNKS(DLLM_DTYPE_F16);
+#undef DLLM_CHUNKS
     if (cudaGetLastError() != cudaSuccess) return DLLM_ERR_CUDA;
     // launched while the chunks run; it waits for them on the GPU
     cudaLaunchAttribute attr = {};
@@ -909,9 +907,7 @@ dllm_status launch_beam_reorder(int batch, int beams, const int32_t *parent, int
     a.slices = (int)slices;
     const int group = (int)(INT32_MAX / per_tensor < RO_TENSORS ? INT32_MAX / per_tensor : RO_TENSORS);
     const size_t smem = (size_t)beams * nt * vb;
-    auto go = [&](auto kernel) {
-        if (cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 131072) != cudaSuccess)
-            return DLLM_ERR_CUDA;
+    auto launch = [&](auto kernel) {
         for (int t = 0; t < ntensors; t += group) {
             const int n = ntensors - t < group ? ntensors - t : group;
             for (int i = 0; i < n; i++) a.tensors[i] = (unsigned char *)tensors[t + i];
@@ -920,9 +916,12 @@ dllm_status launch_beam_reorder(int batch, int beams, const int32_t *parent, int
         }
         return DLLM_OK;
     };
-    if (vb == 16) return go(beam_reorder_kernel<16>);
-    if (vb == 4) return go(beam_reorder_kernel<4>);
-    return go(beam_reorder_kernel<1>);
+    const cudaFuncAttribute size = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    cudaError_t e = vb == 16  ? set_once<beam_reorder_kernel<16>>(size, 131072)
+                    : vb == 4 ? set_once<beam_reorder_kernel<4>>(size, 131072)
+                              : set_once<beam_reorder_kernel<1>>(size, 131072);
+    if (e != cudaSuccess) return DLLM_ERR_CUDA;
+    return vb == 16 ? launch(beam_reorder_kernel<16>) : vb == 4 ? launch(beam_reorder_kernel<4>) : launch(beam_reorder_kernel<1>);
 }
 
 }  // namespace dllm

@@ -752,11 +752,11 @@ bool code_map(CUtensorMap *map, const int8_t *base, int rows, int cols, int64_t 
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int sm_count() {
-    int dev = 0, n = 148;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    return n;
+template <auto Kernel>
+dllm_status launch_product(const cudaLaunchConfig_t &cfg, const CUtensorMap &map_a, const CUtensorMap &map_b,
+                           const MmArgs &p) {
+    if (set_once<Kernel>(cudaFuncAttributeMaxDynamicSharedMemorySize, MM_SMEM) != cudaSuccess) return DLLM_ERR_CUDA;
+    return cudaLaunchKernelEx(&cfg, Kernel, map_a, map_b, p) == cudaSuccess ? DLLM_OK : DLLM_ERR_CUDA;
 }
 
 // A warp per row up to 1024 columns; then a CTA, of 256 threads up to 8192 columns, and for the few
@@ -830,30 +830,27 @@ dllm_status launch_matmul_i8(int m, int n, int k, const int8_t *a, int64_t lda, 
     // few tiles: split k over a cluster of up to 8 CTAs, while the SMs suffice and a part has 4 blocks
     int parts = 1;
     while (parts < 8 && tiles * parts * 2 <= sms && kblocks >= parts * 8) parts *= 2;
-    auto go = [&](auto kernel) {
-        if (cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MM_SMEM) != cudaSuccess)
-            return DLLM_ERR_CUDA;
-        cudaLaunchAttribute attr[2] = {};
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(parts > 1 ? (unsigned)(tiles * parts) : (unsigned)(tiles < sms ? tiles : sms));
-        cfg.blockDim = dim3(MM_THREADS);
-        cfg.dynamicSmemBytes = MM_SMEM;
-        cfg.stream = stream;
-        cfg.attrs = attr;
-        if (early_b) {  // launched while the kernel that makes a runs; it waits for it on the GPU
-            attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-            attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-        }
-        if (parts > 1) {
-            attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-            attr[cfg.numAttrs++].val.clusterDim = {(unsigned)parts, 1, 1};
-        }
-        return cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, p) == cudaSuccess ? DLLM_OK : DLLM_ERR_CUDA;
-    };
+    cudaLaunchAttribute attr[2] = {};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(parts > 1 ? (unsigned)(tiles * parts) : (unsigned)(tiles < sms ? tiles : sms));
+    cfg.blockDim = dim3(MM_THREADS);
+    cfg.dynamicSmemBytes = MM_SMEM;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    if (early_b) {  // launched while the kernel that makes a runs; it waits for it on the GPU
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (parts > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs++].val.clusterDim = {(unsigned)parts, 1, 1};
+    }
     const bool cap = softcap > 0.0f;
-#define DLLM_MATMUL(DT)                                                                                   \
-    (parts > 1 ? (cap ? go(matmul_i8_split_kernel<DT, true>) : go(matmul_i8_split_kernel<DT, false>))     \
-               : (cap ? go(matmul_i8_kernel<DT, true>) : go(matmul_i8_kernel<DT, false>)))
+#define DLLM_MATMUL(DT)                                                                      \
+    (parts > 1 ? (cap ? launch_product<matmul_i8_split_kernel<DT, true>>(cfg, map_a, map_b, p)   \
+                      : launch_product<matmul_i8_split_kernel<DT, false>>(cfg, map_a, map_b, p)) \
+               : (cap ? launch_product<matmul_i8_kernel<DT, true>>(cfg, map_a, map_b, p)         \
+                      : launch_product<matmul_i8_kernel<DT, false>>(cfg, map_a, map_b, p)))
     if (out_dtype == DLLM_DTYPE_F32) return DLLM_MATMUL(DLLM_DTYPE_F32);
     if (out_dtype == DLLM_DTYPE_BF16) return DLLM_MATMUL(DLLM_DTYPE_BF16);
     return DLLM_MATMUL(DLLM_DTYPE_F16);

@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "diskllm_cuda.h"
 
 namespace dllm {
@@ -71,6 +73,29 @@ enum : int {
     FAULT_COPY_WAIT = 1,      // CTA 0, after its slice's bulk copy landed
     FAULT_EXCHANGE_WAIT = 2,  // the last CTA, after exchange #1 completed
 };
+
+// Multiprocessors of the current device, asked for once per device.
+inline int sm_count() {
+    static std::atomic<int> known[64];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+    if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+    return n;
+}
+// Sets an attribute of a kernel, once per kernel and device.
+template <auto Kernel>
+inline cudaError_t set_once(cudaFuncAttribute what, int value) {
+    static std::atomic<unsigned long long> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return cudaSuccess;
+    e = cudaFuncSetAttribute((const void *)Kernel, what, value);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return e;
+}
 
 // Launch configuration chosen by the host for one (vocab, dtype, history bound, top-k bound).
 struct LaunchCfg {
