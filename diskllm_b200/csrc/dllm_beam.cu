@@ -4,9 +4,9 @@
 //   cum(b, i) = score_b + x_bi - log(sum over allowed j of exp(x_bj))
 //   rank      = cum / length^alpha; order: rank desc, beam asc, logit desc, id asc
 //
-// Within a beam that order is the order of the logits, so a row is read once: a chunk of it keeps
+// Within a beam that order is the order of the logits, so a row is read once: a piece of it keeps
 // its k best (logit desc, id asc) and its running maximum and exponential sum, and one CTA per
-// sequence joins the chunks.
+// sequence joins the pieces.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -26,8 +26,8 @@ constexpr int BS_WCAP = 512;        // candidates that a warp holds: at least k 
 constexpr int BS_CAP = BS_WARPS * BS_WCAP;
 constexpr uint32_t KEY_NINF = 0x007fffffu;  // order key of -inf
 
-// One chunk's maximum and its exponential sum, relative to sum_base(m).
-struct ChunkSum {
+// One piece's maximum and its exponential sum, relative to sum_base(m).
+struct PieceSum {
     float m;
     float pad;
     double s;
@@ -100,17 +100,6 @@ __device__ __forceinline__ void sort_desc(uint64_t *buf, int n2, int t, int nt, 
         }
 }
 
-// The j-th largest of a warp's 32 keys (j from 1), in every lane.
-__device__ __forceinline__ uint32_t warp_jth(uint32_t key, int j) {
-    uint32_t mx = __reduce_max_sync(0xffffffffu, key);
-    for (int i = 1; i < j; i++) {
-        const uint32_t holders = __ballot_sync(0xffffffffu, key == mx);
-        if ((threadIdx.x & 31) == __ffs(holders) - 1) key = 0;
-        mx = __reduce_max_sync(0xffffffffu, key);
-    }
-    return mx;
-}
-
 // How 16 bytes hold logits.
 template <int DT>
 struct Vec {
@@ -158,61 +147,20 @@ __device__ __forceinline__ float largest(const uint4 (&v)[U]) {
     return max_keep(p.x, p.y);
 }
 
-// Which elements of U vectors are at or above `least`, as bits: element e of fp32 vectors at bit e;
-// of 16-bit ones, the lower element of word w at bit w and the upper one at bit 16 + w.  `least` is
-// rounded down to the type, so a few more may be marked.
-template <int DT, int U>
-__device__ __forceinline__ uint32_t reaching(const uint4 (&v)[U], float least) {
-    uint32_t take = 0;
-    if (DT == DLLM_DTYPE_F32) {
-#pragma unroll
-        for (int e = 0; e < 4 * U; e++) take |= (uint32_t)(__uint_as_float(word_of(v[e / 4], e % 4)) >= least) << e;
-        return take;
-    }
-    uint32_t two;  // -inf is never marked
-    if (DT == DLLM_DTYPE_BF16) two = __bfloat16_as_ushort(__float2bfloat16_rd(fmaxf(least, -3.38953139e38f)));
-    else two = __half_as_ushort(__float2half_rd(fmaxf(least, -65504.0f)));
-    two |= two << 16;
-#pragma unroll
-    for (int w = 0; w < 4 * U; w++) {
-        uint32_t ge;
-        if (DT == DLLM_DTYPE_BF16) asm("set.ge.u32.bf16x2 %0, %1, %2;" : "=r"(ge) : "r"(word_of(v[w / 4], w % 4)), "r"(two));
-        else asm("set.ge.u32.f16x2 %0, %1, %2;" : "=r"(ge) : "r"(word_of(v[w / 4], w % 4)), "r"(two));
-        take |= ge & (0x10001u << w);
-    }
-    return take;
-}
-// the element at a bit of reaching(), and its number in the vectors
-template <int DT, int U>
-__device__ __forceinline__ float element_of(const uint4 (&v)[U], int bit, int *e) {
-    const int w = bit & 15;
-    uint32_t word = word_of(v[0], 0);
-#pragma unroll
-    for (int i = 1; i < 4 * U; i++) word = w == i ? word_of(v[i / 4], i % 4) : word;
-    if (DT == DLLM_DTYPE_F32) {
-        *e = w;
-        return __uint_as_float(word);
-    }
-    const float2 p = pair_of<DT>(make_uint4(word, 0, 0, 0), 0);
-    *e = 2 * w + (bit >> 4);
-    return bit & 16 ? p.y : p.x;
-}
-
 template <int DT>
 __device__ __forceinline__ uint4 ninf_vector() {
     return make_uint4(Vec<DT>::NINF, Vec<DT>::NINF, Vec<DT>::NINF, Vec<DT>::NINF);
 }
 
-// The vector of elements i0 .. of a row, of which some lie outside it: those and masked ones are -inf.
+// The vector of elements i0 .. of a row, of which some lie outside it: those are -inf.
 template <int DT>
-__device__ __noinline__ uint4 edge_vector(const unsigned char *row, const uint32_t *mask, int i0, int V) {
+__device__ __noinline__ uint4 edge_vector(const unsigned char *row, int i0, int V) {
     constexpr int VEC = Vec<DT>::N;
     uint32_t x[4] = {Vec<DT>::NINF, Vec<DT>::NINF, Vec<DT>::NINF, Vec<DT>::NINF};
 #pragma unroll
     for (int e = 0; e < VEC; e++) {
         if (i0 + e < 0 || e >= V - i0) continue;
         const int i = i0 + e;
-        if (mask && !(mask[i >> 5] >> (i & 31) & 1)) continue;
         if (DT == DLLM_DTYPE_F32) x[e % 4] = ((const uint32_t *)row)[i];
         else {
             const uint32_t u = ((const unsigned short *)row)[i];
@@ -222,120 +170,68 @@ __device__ __noinline__ uint4 edge_vector(const unsigned char *row, const uint32
     return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
-// Grid rows x chunks.  A chunk is a range of the row's 16-byte vectors, counted from the row's
-// first byte rounded down to 16 (so any row start is served; the first and the last vector are
-// read by element).  Per tile a thread updates its running maximum and exponential sum, and a warp
-// that holds an element at or above the threshold appends such elements to its own buffer; no
-// barrier is needed between tiles.
-//
-// Threshold: each warp publishes the `top` largest of its lanes' running maxima, which are different
-// elements; the k-th largest of what the 8 warps have published has k elements at or above it
-// (8 top >= 2 k, so it is close to the k-th largest of all lanes' maxima).  A warp publishes after
-// 1, 2, 3, 5, 9, ... tiles, and the first warp then passes the k-th on; older values are lower, so no
-// order between the warps is needed.  A warp whose
-// buffer could overflow sorts it and keeps its k best: their last key is a threshold for all, and
-// what the warp meets later, with larger ids, has to be strictly above it.
-template <int DT, bool MASK>
-__global__ void __launch_bounds__(BS_NT, 4) beam_chunk_kernel(dllm_beam_desc d, int chunks, ChunkSum *sums,
-                                                              uint64_t *cands) {
-    constexpr int VEC = Vec<DT>::N;
-    __shared__ uint64_t buf[BS_CAP];
-    __shared__ uint64_t few[BS_NT];
-    __shared__ volatile uint32_t tops[BS_NT];  // [warp][top]
-    __shared__ uint32_t floor_key;
-    __shared__ float wm[BS_WARPS];
-    __shared__ double ws[BS_WARPS];
-    __shared__ int wcount[BS_WARPS];
-    asm volatile("griddepcontrol.launch_dependents;");
-    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-    const int64_t row = blockIdx.x / chunks;
-    const int part_no = blockIdx.x % chunks;
-    const int V = d.vocab, k = d.k, top = min(32, (k + 3) / 4);
-    const unsigned char *first = (const unsigned char *)d.logits + (size_t)row * d.row_stride * Vec<DT>::ESZ;
-    const int shift = (int)((uintptr_t)first % 16 / Vec<DT>::ESZ);  // elements before the row in its first vector
-    const uint4 *vecs = (const uint4 *)(first - shift * Vec<DT>::ESZ);
-    const uint32_t *mrow = MASK ? d.mask + row * d.mask_stride : nullptr;
-    const int nvec = (int)(((int64_t)V + shift + VEC - 1) / VEC), per = (nvec + chunks - 1) / chunks;
-    const int v0 = per * part_no, v1 = min(v0 + per, nvec);
-    // vectors from here on are not wholly inside the row, or belong to the next chunk
-    const int v_full = min(v1, (int)(((int64_t)V + shift) / VEC));
+// How the rows' tiles are dealt out: CTA g of `ctas` takes the tiles [g W / ctas, (g + 1) W / ctas) of all
+// W = rows x per_row, so that all have the same work wherever rows begin and end.  The part of a row
+// that one CTA takes is a piece; piece i of a row is that of the i-th CTA that takes some of it.
+struct Split {
+    int64_t all;      // W
+    int ctas, per_row;
+    int pieces;       // at most so many of one row
+    __host__ __device__ int64_t begin(int64_t cta) const { return cta * all / ctas; }
+    __host__ __device__ int cta_of(int64_t tile) const { return (int)(((tile + 1) * ctas - 1) / all); }
+};
 
-    // Vector j; masked elements and those outside the row are -inf.  A vector that is wholly masked
-    // is not read.
-    auto load = [&](int j) {
-        if (j >= v1) return ninf_vector<DT>();
-        const int i0 = j * VEC - shift;
-        if (i0 < 0 || i0 > V - VEC) return edge_vector<DT>(first, mrow, i0, V);
-        if (!MASK) return __ldg(vecs + j);
-        const int w = i0 >> 5, o = i0 & 31;
-        const uint32_t lo = __ldg(mrow + w), hi = o + VEC > 32 ? __ldg(mrow + w + 1) : 0;
-        const uint32_t bits = __funnelshift_r(lo, hi, o) & ((1u << VEC) - 1);
-        uint4 v = ninf_vector<DT>();
-        if (bits) v = __ldg(vecs + j);
-        uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            uint32_t keep;
-            if (DT == DLLM_DTYPE_F32) keep = 0u - (bits >> i & 1);
-            else {
-                const uint32_t two = bits >> (2 * i);
-                keep = ((two | two << 15) & 0x10001u) * 0xffffu;
-            }
-            x[i] = (x[i] & keep) | (Vec<DT>::NINF & ~keep);
-        }
-        return make_uint4(x[0], x[1], x[2], x[3]);
-    };
-    uint4 next[BS_U];  // the next tile
-    auto load_tile = [&](int t0) {
-        if (!MASK && t0 + BS_U * BS_NT <= v_full && (t0 > 0 || shift == 0)) {
-#pragma unroll
-            for (int u = 0; u < BS_U; u++) next[u] = __ldg(vecs + t0 + tid + u * BS_NT);
-        } else {
-#pragma unroll
-            for (int u = 0; u < BS_U; u++) next[u] = load(t0 + u * BS_NT + tid);
-        }
-    };
-    load_tile(v0);  // under way while the beam's state is read
-    if (!beam_live(d, row)) return;
-    tops[tid] = 0;
-    if (tid == 0) floor_key = 0;
-    if (tid < BS_WARPS) wcount[tid] = 0;
-    __syncthreads();
+// The warps' published keys: each warp's `top` largest of its lanes' keys.  The k-th largest of them has
+// k lanes' keys at or above it; 8 top >= 2 k (or all are published), so it is close to the k-th largest
+// of all.  Up to 32 published keys (k <= 16) have their five lowest bits replaced by their places, so
+// that all differ and one comparison with each gives a key's rank; a lower threshold only keeps more.
+// A warp may publish again, higher keys, while others read: each value that k entries were seen to
+// reach stays one that k lanes reach.
+struct Tops {
+    uint4 keys[BS_NT / 4];  // [warp][top]
 
-    float m = -INFINITY;   // this thread's maximum so far
-    double s = 0.0;        // its exponential sum, relative to sum_base(m)
-    uint32_t thr = KEY_NINF + 1;   // a candidate's key has to reach it
-    int count = 0;                 // candidates in this warp's buffer
-    uint64_t *mine = buf + wid * BS_WCAP;
-
-    auto publish = [&] {
-        uint32_t key = okey(m);
-        for (int i = 0; i < top; i++) {
+    __device__ __forceinline__ static int top(int k) { return min(32, (k + 3) / 4); }
+    __device__ __forceinline__ void clear() {
+        if (threadIdx.x < BS_NT / 4) keys[threadIdx.x] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void publish(uint32_t key, int k) {
+        const int lane = threadIdx.x & 31, n = top(k);
+        volatile uint32_t *mine = (volatile uint32_t *)keys + (threadIdx.x >> 5) * n;
+        for (int i = 0; i < n; i++) {
             const uint32_t mx = __reduce_max_sync(0xffffffffu, key);
             const uint32_t holders = __ballot_sync(0xffffffffu, key == mx);
             if (lane == __ffs(holders) - 1) {
-                tops[wid * top + i] = mx;
+                mine[i] = k <= 16 ? (mx & ~31u) | (31 - ((threadIdx.x >> 5) * n + i)) : mx;
                 key = 0;
             }
         }
-    };
-    // The k-th largest published key, without its five lowest bits: they make the keys of a lane
-    // group different, so that one comparison with each gives a key's place.
-    auto kth_published = [&] {
+        __syncwarp();
+    }
+    // the k-th largest, or 0 where none was found
+    __device__ __forceinline__ uint32_t kth(int k) const {
+        const int lane = threadIdx.x & 31, n = BS_WARPS * top(k);
         uint32_t found = 0;
-        if (k <= 16) {  // 32 keys at most
-            const uint32_t v = lane < BS_WARPS * top ? tops[lane] & ~31u | (31 - lane) : 0;
+        if (k <= 16) {
+            const uint32_t v = lane < n ? ((volatile const uint32_t *)keys)[lane] : 0;
+            const uint32_t at = (uint32_t)__cvta_generic_to_shared(keys);
             int above = 0;
-#pragma unroll 8
-            for (int i = 0; i < BS_WARPS * top; i++) above += (tops[i] & ~31u | (31 - i)) > v;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {  // places past the last published one hold 0
+                uint4 o;
+                asm volatile("ld.volatile.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(o.x), "=r"(o.y), "=r"(o.z), "=r"(o.w)
+                             : "r"(at + 16 * i));
+                above += (o.x > v) + (o.y > v) + (o.z > v) + (o.w > v);
+            }
             if (above == k - 1) found = v & ~31u;
         } else {
-            for (int at = lane; at < BS_WARPS * top; at += 32) {
-                const uint32_t v = tops[at];
+            volatile const uint32_t *all = (volatile const uint32_t *)keys;
+            for (int at = lane; at < n; at += 32) {
+                const uint32_t v = all[at];
                 int above = 0, same = 0;
 #pragma unroll 8
-                for (int i = 0; i < BS_WARPS * top; i++) {
-                    const uint32_t o = tops[i];
+                for (int i = 0; i < n; i++) {
+                    const uint32_t o = all[i];
                     above += o > v;
                     same += o == v;
                 }
@@ -343,67 +239,236 @@ __global__ void __launch_bounds__(BS_NT, 4) beam_chunk_kernel(dllm_beam_desc d, 
             }
             __syncwarp();
         }
-        // warps go on publishing meanwhile, so a lane may find none, or another one; each is a key
-        // that k elements reach
         return __reduce_max_sync(0xffffffffu, found);
-    };
-    // this warp's k best, sorted
-    auto cut = [&] {
-        for (int i = count + lane; i < BS_WCAP; i += 32) mine[i] = 0;
-        __syncwarp();
-        sort_desc(mine, BS_WCAP, lane, 32, [] { __syncwarp(); });
+    }
+};
+
+template <int DT>
+__device__ __forceinline__ float load_one(const void *row, int i) {
+    if (DT == DLLM_DTYPE_F32) return __ldg((const float *)row + i);
+    const unsigned short u = __ldg((const unsigned short *)row + i);
+    return DT == DLLM_DTYPE_BF16 ? __uint_as_float((uint32_t)u << 16) : __half2float(__ushort_as_half(u));
+}
+
+// A warp sorts its candidates, best first; the k-th.
+__device__ __noinline__ uint64_t warp_sorts(uint64_t *mine, int count, int k) {
+    const int lane = threadIdx.x & 31;
+    for (int i = count + lane; i < BS_WCAP; i += 32) mine[i] = 0;
+    __syncwarp();
+    sort_desc(mine, BS_WCAP, lane, 32, [] { __syncwarp(); });
+    return mine[k - 1];
+}
+
+// A CTA's shared memory for one piece of a row.
+struct PieceShared {
+    uint64_t buf[BS_CAP];          // [warp][BS_WCAP] candidates
+    uint64_t few[BS_NT];
+    Tops tops;
+    uint32_t floor_key;
+    int wcount[BS_WARPS];
+    float wm[BS_WARPS];
+    double ws[BS_WARPS];
+};
+
+// What a thread keeps of its piece: the running maximum and exponential sum of its elements, and its
+// warp's candidates.
+//
+// Threshold: the k-th of the warps' published keys, of their lanes' running maxima, which are different
+// elements.  While candidates are taken as they come, a warp publishes after 2^i of its tiles, and the
+// first warp passes the k-th on a tile later; older values are lower, so no order between the warps is
+// needed, and no barrier.  A warp whose buffer could overflow sorts it and keeps its k best: their last
+// key is a threshold for all, and the warp itself then takes only what comes before the last of them.
+struct Piece {
+    PieceShared &sh;
+    const int lane, wid, k;
+    uint64_t *const mine;    // this warp's candidates
+    int count = 0;           // how many they are
+    uint32_t thr = KEY_NINF + 1;   // a candidate's key has to reach it
+    uint64_t last = 0;             // and the candidate has to come before this one
+    float m = -INFINITY;     // this thread's maximum so far
+    float base = -INFINITY;  // (float)sum_base(m)
+    double s = 0.0;          // its exponential sum, relative to sum_base(m)
+    int tile = 0;
+
+    __device__ __forceinline__ Piece(PieceShared &shared, int k_)
+        : sh(shared), lane(threadIdx.x & 31), wid(threadIdx.x >> 5), k(k_),
+          mine(shared.buf + (threadIdx.x >> 5) * BS_WCAP) {
+        __syncthreads();  // the piece before is done with the shared memory
+        sh.tops.clear();
+        if (threadIdx.x == 0) sh.floor_key = 0;
+        __syncthreads();
+    }
+    // keeps this warp's k best
+    __device__ __forceinline__ void cut() {
+        const uint64_t kth = warp_sorts(mine, count, k);
         if (count >= k) {
             count = k;
-            const uint32_t last = (uint32_t)(mine[k - 1] >> 32);
-            if (lane == 0) atomicMax(&floor_key, last);
-            thr = max(thr, last + 1);
+            last = kth;
+            thr = max(thr, (uint32_t)(last >> 32));
+            if (lane == 0) atomicMax(&sh.floor_key, (uint32_t)(last >> 32));
         }
-        if (lane == 0) wcount[wid] = count;
         __syncwarp();
-    };
-
-    // appends the elements of a tile that reach the threshold
-    auto collect = [&](const uint4 (&x)[BS_U], int t0) {
-        const uint32_t all = reaching<DT, BS_U>(x, okey_value(thr));
-        auto append = [&](uint32_t take) {
-            while (take) {
-                const int bit = __ffs(take) - 1;
-                take &= take - 1;
-                int e;  // element of this thread's tile: vector e / VEC, place e % VEC
-                const uint32_t key = okey(element_of<DT, BS_U>(x, bit, &e));
-                if (key >= thr)
-                    mine[atomicAdd(&wcount[wid], 1)] =
-                        composite(key, (t0 + e / VEC * BS_NT + tid) * VEC - shift + e % VEC);
+    }
+    // the lanes' elements x, of those that have one, if they can be among the k best
+    __device__ __forceinline__ void offer(bool has, float x, int id) {
+        const uint32_t key = okey(x);
+        const uint64_t c = composite(key, id);
+        const bool take = has && x == x && key >= thr && c > last;
+        const uint32_t who = __ballot_sync(0xffffffffu, take);
+        if (take) mine[count + __popc(who & ((1u << lane) - 1))] = c;
+        count += __popc(who);
+        if (count > BS_WCAP - 32) cut();
+    }
+    // The maximum and the reference of the sum after a tile whose largest element is `tm`; false where some
+    // lane's lies beyond the range in which sum_base is one rounded product.
+    __device__ __forceinline__ bool raise(float tm) {
+        const float to = max_keep(m, tm);
+        const bool plain = !__any_sync(0xffffffffu, fabsf(to) >= BASE_EXACT && to > -INFINITY);
+        if (plain) {
+            if (tm > m) {
+                const float b = __fmul_rn(tm, LOG2E);
+                s *= (double)exp2_approx(__fsub_rn(base, b));
+                base = b;
             }
-            __syncwarp();
-            count = *(volatile int *)&wcount[wid];
-        };
-        if (count + __reduce_add_sync(0xffffffffu, __popc(all)) <= BS_WCAP) append(all);
-        else
-#pragma unroll 1
-            for (int u = 0; u < BS_U; u++) {  // one vector of each lane at a time
-                if (count > BS_WCAP - 32 * VEC) cut();
-                append(all & (DT == DLLM_DTYPE_F32 ? 0xfu : 0xf000fu) << (4 * u));
-            }
-    };
-
-    float base = -INFINITY;  // sum_base(m), for |m| < 2^20
-    int tile = 0;
-    for (int t0 = v0; t0 < v1; t0 += BS_NT * BS_U, tile++) {
-        uint4 x[BS_U];
+        } else if (tm > m) {
+            s *= rebase(m, tm);
+            base = (float)sum_base(tm);
+        }
+        m = to;
+        return plain;
+    }
+    __device__ __forceinline__ float plain_base() const { return m == -INFINITY ? 0.0f : base; }
+    // exponent of x where raise() gave false, as x - ref and what is added to LOG2E times that
+    __device__ __forceinline__ void exact_base(float *ref, float *off) const {
+        *ref = m == -INFINITY ? 0.0f : m;
+        *off = (float)((double)LOG2E * (double)*ref - sum_base(*ref));
+    }
+    // all warps, after their first tile: a threshold that k elements reach
+    __device__ __forceinline__ void settle_threshold() {
+        sh.tops.publish(okey(m), k);
+        __syncthreads();
+        thr = max(thr, sh.tops.kth(k));
+    }
+    // after tile number `tile` (from 1), where candidates are taken as they come: their threshold
+    __device__ __forceinline__ void raise_threshold() {
+        if ((tile & (tile - 1)) == 0) sh.tops.publish(okey(m), k);
+        if (wid == 0 && ((tile - 1) & (tile - 2)) == 0) {  // a tile later, when the others have published too
+            const uint32_t kth = sh.tops.kth(k);
+            if (lane == 0) atomicMax(&sh.floor_key, kth);
+        }
+        thr = max(thr, *(volatile uint32_t *)&sh.floor_key);
+    }
+    // all warps: the piece's maximum, sum and k best
+    __device__ __forceinline__ void finish(PieceSum *sum, uint64_t *out) {
+        const float M_warp = okey_value(__reduce_max_sync(0xffffffffu, m == m ? okey(m) : 0xffffffffu));
+        if (lane == 0) {
+            sh.wm[wid] = M_warp;
+            sh.wcount[wid] = count;
+        }
+        __syncthreads();
+        float M = sh.wm[0];
+        int n = 0, at = 0;
 #pragma unroll
-        for (int u = 0; u < BS_U; u++) x[u] = next[u];
-        load_tile(t0 + BS_NT * BS_U);
+        for (int w = 0; w < BS_WARPS; w++) {
+            M = max_keep(M, sh.wm[w]);
+            if (w == wid) at = n;
+            n += sh.wcount[w];
+        }
+        double S = s * rebase(m, M);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) S += __shfl_xor_sync(0xffffffffu, S, o);
+        if (lane == 0) sh.ws[wid] = S;
+        if (n > BS_NT) {  // leave those that reach the last threshold
+            sh.tops.publish(okey(m), k);
+            __syncthreads();
+            const uint64_t lowest = (uint64_t)max(sh.tops.kth(k), sh.floor_key) << 32;
+            int kept = 0;
+            for (int i = lane; i < (count + 31) / 32 * 32; i += 32) {  // in place: what is kept moves to the front
+                const uint64_t c = i < count ? mine[i] : 0;
+                const bool keep = i < count && c >= lowest;
+                const uint32_t who = __ballot_sync(0xffffffffu, keep);
+                if (keep) mine[kept + __popc(who & ((1u << lane) - 1))] = c;
+                kept += __popc(who);
+            }
+            count = kept;
+            if (lane == 0) sh.wcount[wid] = kept;
+            __syncthreads();
+            n = 0;
+#pragma unroll
+            for (int w = 0; w < BS_WARPS; w++) {
+                if (w == wid) at = n;
+                n += sh.wcount[w];
+            }
+        }
+        const int tid = threadIdx.x;
+        if (n <= BS_NT) {  // each candidate's place is the number of larger ones
+            for (int i = lane; i < count; i += 32) sh.few[at + i] = mine[i];
+            __syncthreads();
+            if (tid < n) {
+                const uint64_t c = sh.few[tid];
+                int place = 0;
+#pragma unroll 4
+                for (int i = 0; i < n; i++) place += sh.few[i] > c;
+                if (place < k) out[place] = c;
+            }
+            for (int i = n + tid; i < k; i += BS_NT) out[i] = 0;
+        } else {
+            for (int i = count + lane; i < BS_WCAP; i += 32) mine[i] = 0;
+            __syncthreads();
+            sort_desc(sh.buf, BS_CAP, tid, BS_NT, [] { __syncthreads(); });
+            for (int i = tid; i < k; i += BS_NT) out[i] = sh.buf[i];
+        }
+        if (tid == 0) {
+            double total = 0.0;
+#pragma unroll
+            for (int w = 0; w < BS_WARPS; w++) total += sh.ws[w];
+            *sum = {M, 0.0f, total};
+        }
+    }
+};
+
+// Pieces of rows without a mask.  A tile is BS_NT * BS_U of the row's 16-byte vectors, counted from the
+// row's first byte rounded down to 16 (so any row start is served; the first and the last vector are
+// read by element).  The next tile is loaded while one is worked on.
+template <int DT>
+__device__ __forceinline__ void dense_piece(const dllm_beam_desc &d, PieceShared &sh, int64_t row, int tile0, int ntiles,
+                                            PieceSum *sum, uint64_t *out) {
+    constexpr int VEC = Vec<DT>::N, TILE = BS_NT * BS_U;
+    const int tid = threadIdx.x;
+    const int V = d.vocab;
+    const unsigned char *first = (const unsigned char *)d.logits + (size_t)row * d.row_stride * Vec<DT>::ESZ;
+    const int shift = (int)((uintptr_t)first % 16 / Vec<DT>::ESZ);  // elements before the row in its first vector
+    const uint4 *vecs = (const uint4 *)(first - shift * Vec<DT>::ESZ);
+    const int nvec = (int)(((int64_t)V + shift + VEC - 1) / VEC), v0 = tile0 * TILE, v1 = min(v0 + ntiles * TILE, nvec);
+    // vectors from here on are not wholly inside the row, or belong to the next piece
+    const int v_full = min(v1, (int)(((int64_t)V + shift) / VEC));
+
+    auto load = [&](uint4 (&x)[BS_U], int t0) {
+        if (t0 + TILE <= v_full && (t0 > 0 || shift == 0)) {
+#pragma unroll
+            for (int u = 0; u < BS_U; u++) x[u] = __ldg(vecs + t0 + tid + u * BS_NT);
+        } else {
+#pragma unroll
+            for (int u = 0; u < BS_U; u++) {
+                const int j = t0 + tid + u * BS_NT;
+                x[u] = ninf_vector<DT>();
+                if (j >= v1) continue;
+                if (j < v_full && (j > 0 || shift == 0)) x[u] = __ldg(vecs + j);
+                else x[u] = edge_vector<DT>(first, j * VEC - shift, V);
+            }
+        }
+    };
+    uint4 x[BS_U], next[BS_U];
+    load(next, v0);  // under way while the beam's state is read
+    if (!beam_live(d, row)) return;
+    Piece c(sh, d.k);
+
+    auto work = [&](const uint4 (&x)[BS_U]) {
         const float tm = largest<DT, BS_U>(x);
         Pair part(0.0f, 0.0f);
         const Pair scale(LOG2E, LOG2E);
-        if (!__any_sync(0xffffffffu, fabsf(tm) >= BASE_EXACT || fabsf(m) >= BASE_EXACT)) {
-            if (tm > m) {
-                const float to = __fmul_rn(tm, LOG2E);
-                s *= (double)exp2_approx(__fsub_rn(base, to));
-                base = to;
-                m = tm;
-            }
+        if (c.raise(tm)) {
+            const float base = c.plain_base();
             const Pair minus(-base, -base);
 #pragma unroll
             for (int u = 0; u < BS_U; u++)
@@ -412,13 +477,9 @@ __global__ void __launch_bounds__(BS_NT, 4) beam_chunk_kernel(dllm_beam_desc d, 
                     const float2 xi = pair_of<DT>(x[u], i);
                     part = add2(part, exp2_approx(fma2(Pair(xi.x, xi.y), scale, minus)));
                 }
-        } else {  // values from 2^20 on, or nothing above -inf yet
-            if (tm > m) {
-                s *= rebase(m, tm);
-                m = tm;
-            }
-            base = m == -INFINITY ? m : (float)sum_base(m);
-            const float ref = m == -INFINITY ? 0.0f : m, off = (float)((double)LOG2E * (double)ref - sum_base(ref));
+        } else {
+            float ref, off;
+            c.exact_base(&ref, &off);
 #pragma unroll 1
             for (int u = 0; u < BS_U; u++) {
                 uint4 xu = x[0];
@@ -432,79 +493,164 @@ __global__ void __launch_bounds__(BS_NT, 4) beam_chunk_kernel(dllm_beam_desc d, 
                 }
             }
         }
-        s += (double)part.sum();
+        c.s += (double)part.sum();
+        return tm;
+    };
+    // the warp looks at one lane's vector together, an element in each lane
+    auto offer_vector = [&](const uint4 &v, int holder, int j) {
+        const int e = c.lane % VEC;
+        const uint4 o = make_uint4(__shfl_sync(0xffffffffu, v.x, holder), __shfl_sync(0xffffffffu, v.y, holder),
+                                   __shfl_sync(0xffffffffu, v.z, holder), __shfl_sync(0xffffffffu, v.w, holder));
+        float f;
+        if (DT == DLLM_DTYPE_F32) f = __uint_as_float(word_of(o, e));
+        else {
+            const float2 pr = pair_of<DT>(make_uint4(word_of(o, e / 2), 0, 0, 0), 0);
+            f = e & 1 ? pr.y : pr.x;
+        }
+        c.offer(c.lane < VEC, f, j * VEC - shift + e);
+    };
+    auto holders_of = [&](const uint4 &v) {
+        const uint4 one[1] = {v};
+        return __ballot_sync(0xffffffffu, largest<DT, 1>(one) >= okey_value(c.thr));
+    };
+    for (int t0 = v0;;) {
+#pragma unroll
+        for (int u = 0; u < BS_U; u++) x[u] = next[u];
+        load(next, t0 + TILE);
+        const float tm = work(x);
+        c.tile++;
+        if (c.tile == 1) c.settle_threshold();  // with every warp's first tile
+        else c.raise_threshold();
+        if (__any_sync(0xffffffffu, tm >= okey_value(c.thr)))
+#pragma unroll
+            for (int u = 0; u < BS_U; u++)
+                for (uint32_t hit = holders_of(x[u]); hit; hit &= hit - 1)
+                    offer_vector(x[u], __ffs(hit) - 1, t0 + u * BS_NT + c.wid * 32 + __ffs(hit) - 1);
+        t0 += TILE;
+        if (t0 >= v1) break;
+    }
+    c.finish(sum, out);
+}
 
-        if ((tile & (tile - 1)) == 0) {  // after 1, 2, 3, 5, 9, ... tiles
-            publish();
-            if (tile == 0) {  // the first threshold is taken from every warp's first tile
-                __syncthreads();
-                thr = max(thr, kth_published());
-            } else if (wid == 0) {
-                __syncwarp();
-                const uint32_t kth = kth_published();
-                if (lane == 0) atomicMax(&floor_key, kth);
+// Pieces of rows with a mask.  A tile is BS_NT of the row's mask words, a warp takes 32 words (1024 ids) at
+// a time, and only allowed logits are read.  Where at most a quarter of the 1024 is allowed each lane
+// takes the set bits of its own word, four a round; else the warp takes four words a round, a bit of
+// them each lane.  Logits are read singly, so rows may start anywhere.
+template <int DT>
+__device__ __forceinline__ void masked_piece(const dllm_beam_desc &d, PieceShared &sh, int64_t row, int tile0, int ntiles,
+                                             PieceSum *sum, uint64_t *out) {
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+    const int V = d.vocab, words = (int)(((int64_t)V + 31) / 32), w0 = tile0 * BS_NT, w1 = min(w0 + ntiles * BS_NT, words);
+    const uint32_t *mask = d.mask + row * d.mask_stride;
+    const unsigned char *logits = (const unsigned char *)d.logits + (size_t)row * d.row_stride * Vec<DT>::ESZ;
+    auto word_at = [&](int i) {
+        if (i >= w1) return 0u;
+        const uint32_t w = __ldg(mask + i);
+        return i == words - 1 && (V & 31) ? w & ((1u << (V & 31)) - 1) : w;
+    };
+    int group = w0 + wid * 32;  // this warp's words
+    uint32_t word = word_at(group + lane), next_word = word_at(group + 32 * BS_WARPS + lane);
+    if (!beam_live(d, row)) return;
+    Piece c(sh, d.k);
+
+    // Four elements of a lane: element e has the id start + (places >> 8 e & 255); absent ones are -inf.
+    struct Round {
+        float x[4];
+        int start;
+        uint32_t places;
+    };
+    int dense_at = -1;  // word of the group that a dense group's next round starts at; -1: not dense
+    bool fresh = true;
+    auto fetch = [&](Round &r) {
+        for (;;) {
+            if (fresh) {
+                fresh = false;
+                dense_at = __reduce_add_sync(0xffffffffu, __popc(word)) > 256 ? 0 : -1;
+            }
+            if (dense_at >= 0 ? dense_at < 32 : __any_sync(0xffffffffu, word)) break;
+            group += 32 * BS_WARPS;
+            if (group >= w1) return false;
+            word = next_word;
+            next_word = word_at(group + 32 * BS_WARPS + lane);
+            fresh = true;
+        }
+        bool has[4];
+        r.places = 0;
+        if (dense_at >= 0) {
+            r.start = (group + dense_at) * 32 + lane;
+            r.places = 0u | 32u << 8 | 64u << 16 | 96u << 24;
+#pragma unroll
+            for (int e = 0; e < 4; e++) has[e] = __shfl_sync(0xffffffffu, word, dense_at + e) >> lane & 1;
+            dense_at += 4;
+        } else {
+            r.start = (group + lane) * 32;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                has[e] = word != 0;
+                r.places |= (uint32_t)((__ffs(word) - 1) & 255) << (8 * e);
+                word &= word - 1;
             }
         }
-        thr = max(thr, *(volatile uint32_t *)&floor_key);
-        if (__any_sync(0xffffffffu, tm >= okey_value(thr))) collect(x, t0);
-    }
-
-    // the chunk's maximum and sum, and the warps' candidates that reach the last threshold
-    float M = m;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) M = max_keep(M, __shfl_xor_sync(0xffffffffu, M, o));
-    publish();
-    if (lane == 0) wm[wid] = M;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < BS_WARPS; w++) M = max_keep(M, wm[w]);
-    double S = s * rebase(m, M);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) S += __shfl_xor_sync(0xffffffffu, S, o);
-    const uint64_t lowest = (uint64_t)max(kth_published(), floor_key) << 32;
-    int kept = 0;
-    for (int i = lane; i < (count + 31) / 32 * 32; i += 32) {  // in place: what is kept moves towards the front
-        const uint64_t c = i < count ? mine[i] : 0;
-        const bool keep = i < count && c >= lowest;
-        const uint32_t who = __ballot_sync(0xffffffffu, keep);
-        if (keep) mine[kept + __popc(who & ((1u << lane) - 1))] = c;
-        kept += __popc(who);
-    }
-    if (lane == 0) {
-        ws[wid] = S;
-        wcount[wid] = kept;
-    }
-    __syncthreads();
-    int n = 0, at = 0;
-#pragma unroll
-    for (int w = 0; w < BS_WARPS; w++) {
-        if (w == wid) at = n;
-        n += wcount[w];
-    }
-    const int64_t chunk = blockIdx.x;
-    if (tid == 0) {
-        double tot = 0.0;
-        for (int w = 0; w < BS_WARPS; w++) tot += ws[w];
-        sums[chunk] = {M, 0.0f, tot};
-    }
-    uint64_t *out = cands + chunk * k;
-    if (n <= BS_NT) {  // each candidate's place is the number of larger ones
-        for (int i = lane; i < kept; i += 32) few[at + i] = mine[i];
-        __syncthreads();
-        if (tid < n) {
-            const uint64_t c = few[tid];
-            int place = 0;
-            for (int i = 0; i < n; i++) place += few[i] > c;
-            if (place < k) out[place] = c;
+        for (int e = 0; e < 4; e++) {
+            const int i = r.start + (int)(r.places >> (8 * e) & 255);
+            r.x[e] = has[e] ? load_one<DT>(logits, i) : -INFINITY;
         }
-        for (int i = n + tid; i < k; i += BS_NT) out[i] = 0;
-        return;
+        return true;
+    };
+    auto work = [&](const Round &r) {
+        const float tm = max_keep(max_keep(r.x[0], r.x[1]), max_keep(r.x[2], r.x[3]));
+        float part = 0.0f;
+        if (c.raise(tm)) {
+            const float base = c.plain_base();
+#pragma unroll
+            for (int e = 0; e < 4; e++) part += exp2_approx(__fmaf_rn(r.x[e], LOG2E, -base));
+        } else {
+            float ref, off;
+            c.exact_base(&ref, &off);
+#pragma unroll
+            for (int e = 0; e < 4; e++) part += exp2_approx(__fmaf_rn(r.x[e] - ref, LOG2E, off));
+        }
+        c.s += (double)part;
+        c.tile++;
+        if (c.tile == 1) c.settle_threshold();  // with every warp's first round
+        else c.raise_threshold();
+        if (!__any_sync(0xffffffffu, tm >= okey_value(c.thr))) return;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            c.offer(r.x[e] >= okey_value(c.thr), r.x[e], r.start + (int)(r.places >> (8 * e) & 255));
+    };
+    Round a, b;
+    bool more = group < w1 && fetch(a);
+    if (!more) c.settle_threshold();  // no allowed id here: the warp still joins the others
+    while (more) {
+        more = fetch(b);
+        work(a);
+        if (!more) break;
+        more = fetch(a);
+        work(b);
     }
-    for (int i = kept + lane; i < BS_WCAP; i += 32) mine[i] = 0;
-    __syncthreads();
-    sort_desc(buf, BS_CAP, tid, BS_NT, [] { __syncthreads(); });
-    for (int i = tid; i < k; i += BS_NT) out[i] = buf[i];
+    c.finish(sum, out);
 }
+
+// Persistent, 3 or 4 CTAs per SM: each takes its share of the tiles, piece by piece.
+template <int DT, bool MASK>
+__global__ void __launch_bounds__(BS_NT, MASK ? 4 : 3) beam_pieces_kernel(dllm_beam_desc d, Split split, PieceSum *sums,
+                                                                          uint64_t *cands) {
+    __shared__ PieceShared sh;
+    asm volatile("griddepcontrol.launch_dependents;");
+    int64_t at = split.begin(blockIdx.x);
+    const int64_t end = split.begin(blockIdx.x + 1);
+    while (at < end) {
+        const int64_t row = at / split.per_row;
+        const int tile = (int)(at - row * split.per_row), n = (int)min((int64_t)(split.per_row - tile), end - at);
+        const int64_t piece = row * split.pieces + ((int)blockIdx.x - split.cta_of(row * split.per_row));
+        if (MASK) masked_piece<DT>(d, sh, row, tile, n, sums + piece, cands + piece * d.k);
+        else dense_piece<DT>(d, sh, row, tile, n, sums + piece, cands + piece * d.k);
+        at += n;
+    }
+}
+
 
 struct Best {
     double rank;
@@ -523,8 +669,8 @@ __device__ __forceinline__ bool before(const Best &a, const Best &b) {
     return a.comp > b.comp;
 }
 
-// One CTA per sequence: the beams' log-sum-exps from their chunks, then the k best of the chunks'
-// candidates.  The same threshold as in a chunk (over the threads' best ranks, rounded down to
+// One CTA per sequence: the beams' log-sum-exps from their pieces, then the k best of the pieces'
+// candidates.  The same threshold as in a piece (over the threads' best ranks, rounded down to
 // fp32, which keeps their order) leaves a few; each one's place is the number that comes before
 // it.  Where more are left than fit, the threshold is raised to the highest that k candidates
 // reach; where that still leaves too many (equal ranks), k rounds take the best candidate that
@@ -532,8 +678,9 @@ __device__ __forceinline__ bool before(const Best &a, const Best &b) {
 constexpr int BM_LEFT = 512;
 constexpr int BM_HELD = 4;  // candidates that a thread keeps in registers
 
-__global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, const ChunkSum *sums,
-                                                           const uint64_t *cands, int chunks) {
+__global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, const PieceSum *sums,
+                                                           const uint64_t *cands, Split split) {
+    __shared__ int npieces[DLLM_BEAM_MAX];
     __shared__ double lse[DLLM_BEAM_MAX], inv_len[DLLM_BEAM_MAX];
     __shared__ float score_in[DLLM_BEAM_MAX];  // copies, so that the outputs may lie over the inputs
     __shared__ int length_in[DLLM_BEAM_MAX];
@@ -541,19 +688,22 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
     __shared__ Best wbest[BS_WARPS];
     __shared__ uint64_t left_key[BM_LEFT], left_comp[BM_LEFT];
     __shared__ int left_beam[BM_LEFT];
-    __shared__ uint32_t wkey[BS_WARPS];
+    __shared__ Tops tops;
+    __shared__ int wnumber[BS_WARPS];
     __shared__ int nleft;
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const int K = d.beams, k = d.k;
     const int64_t item = blockIdx.x;
     if (tid == 0) nleft = 0;
-    // what does not come from the chunks is read while they run
+    tops.clear();
+    // what does not come from the pieces is read while they run
     for (int b = tid; b < K; b += BS_NT) {
         const int64_t row = item * K + b;
         const float sc = d.scores[row];
         const bool ended = d.finished && d.finished[row];
         const int len_in = d.lengths ? d.lengths[row] : 0;
         const double len = fmax((double)len_in + (ended ? 0.0 : 1.0), 1.0);
+        npieces[b] = split.cta_of((row + 1) * split.per_row - 1) - split.cta_of(row * split.per_row) + 1;
         length_in[b] = len_in;
         score_in[b] = sc;
         inv_len[b] = d.length_penalty != 0.0f && d.lengths ? 1.0 / pow(len, (double)d.length_penalty) : 1.0;
@@ -561,18 +711,20 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
     }
     __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int per_beam = chunks * k, N = K * per_beam;
+    const int lists = split.pieces, per_beam = lists * k, N = K * per_beam;
     const uint64_t *mine = cands + item * N;
-    // The warps take the chunks' lists in turn, so that each meets every beam's candidates: their
-    // thresholds are then alike.  Candidate number q of a warp is position q % k of its list q / k.
-    const int warp_n = ((K * chunks - wid + BS_WARPS - 1) / BS_WARPS) * k;
+    // The warps take the pieces' lists in turn, so that the best are spread over them.  Candidate number q of a warp is position q % k of its list q / k.
+    const int warp_n = ((K * lists - wid + BS_WARPS - 1) / BS_WARPS) * k;
     auto number = [&](int q) { return q < warp_n ? ((q / k) * BS_WARPS + wid) * k + q % k : N; };
+    auto comp_at = [&](int e, int b) {  // a beam that offers none, or a piece that is not there, has none
+        return live[b] == 1 && e / k - b * lists < npieces[b] ? mine[e] : 0;
+    };
     uint64_t held[BM_HELD];  // this thread's first candidates
     int at_e[BM_HELD];
 #pragma unroll
     for (int i = 0; i < BM_HELD; i++) {
         const int e = at_e[i] = number(lane + 32 * i);
-        held[i] = e < N && live[e / per_beam] == 1 ? mine[e] : 0;
+        held[i] = e < N ? comp_at(e, e / per_beam) : 0;
     }
     for (int b = wid; b < K; b += BS_WARPS) {
         const int64_t row = item * K + b;
@@ -582,20 +734,18 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
         if (kind == 1) {
             float M = -INFINITY;
             double S = 0.0;
-            if (chunks <= 32) {
-                const ChunkSum p = lane < chunks ? sums[row * chunks + lane] : ChunkSum{-INFINITY, 0.0f, 0.0};
+            const PieceSum *mysums = sums + row * lists;
+            if (npieces[b] <= 32) {
+                const PieceSum p = lane < npieces[b] ? mysums[lane] : PieceSum{-INFINITY, 0.0f, 0.0};
                 M = p.m;
 #pragma unroll
                 for (int o = 16; o; o >>= 1) M = max_keep(M, __shfl_xor_sync(0xffffffffu, M, o));
                 S = p.s * rebase(p.m, M);
             } else {
-                for (int c = lane; c < chunks; c += 32) M = max_keep(M, sums[row * chunks + c].m);
+                for (int c = lane; c < npieces[b]; c += 32) M = max_keep(M, mysums[c].m);
 #pragma unroll
                 for (int o = 16; o; o >>= 1) M = max_keep(M, __shfl_xor_sync(0xffffffffu, M, o));
-                for (int c = lane; c < chunks; c += 32) {
-                    const ChunkSum p = sums[row * chunks + c];
-                    S += p.s * rebase(p.m, M);
-                }
+                for (int c = lane; c < npieces[b]; c += 32) S += mysums[c].s * rebase(mysums[c].m, M);
             }
 #pragma unroll
             for (int o = 16; o; o >>= 1) S += __shfl_xor_sync(0xffffffffu, S, o);
@@ -613,7 +763,7 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
         }
     }
     __syncthreads();
-    // candidate e: position e % k of a chunk's list; an ended beam offers its first position only
+    // candidate e: position e % k of a piece's list; an ended beam offers its first position only
     auto candidate_of = [&](int e, int b, uint64_t comp, Best *c) {
         double cum = (double)score_in[b];
         if (live[b] == 0) return false;
@@ -629,7 +779,7 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
     };
     auto candidate = [&](int e, Best *c) {
         const int b = e / per_beam;
-        return candidate_of(e, b, live[b] == 1 ? mine[e] : 0, c);
+        return candidate_of(e, b, comp_at(e, b), c);
     };
     auto emit = [&](int place, const Best &c, bool none) {
         float score = -INFINITY;
@@ -663,12 +813,9 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
         Best c;
         if (candidate(number(q), &c)) mx = max(mx, okey(__double2float_rd(c.rank)));
     }
-    const uint32_t kj = warp_jth(mx, (k + BS_WARPS - 1) / BS_WARPS);
-    if (lane == 0) wkey[wid] = kj;
+    tops.publish(mx, k);
     __syncthreads();
-    uint32_t lo = wkey[0];
-#pragma unroll
-    for (int w = 1; w < BS_WARPS; w++) lo = min(lo, wkey[w]);
+    const uint32_t lo = tops.kth(k);
 #pragma unroll
     for (int i = 0; i < BM_HELD; i++) {
         if (key[i] == 0 || key[i] < lo) continue;
@@ -695,11 +842,11 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
             }
             c_mid = __reduce_add_sync(0xffffffffu, c_mid);
             __syncthreads();
-            if (lane == 0) wkey[wid] = c_mid;
+            if (lane == 0) wnumber[wid] = c_mid;
             __syncthreads();
             c_mid = 0;
 #pragma unroll
-            for (int w = 0; w < BS_WARPS; w++) c_mid += wkey[w];
+            for (int w = 0; w < BS_WARPS; w++) c_mid += wnumber[w];
             if (c_mid >= k) reached = mid;
             else above = mid;
         }
@@ -760,21 +907,20 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
     }
 }
 
-// Chunks per row: the count whose waves of CTAs (4 per SM) take least, a chunk's set-up and
-// selection counted as two tiles.
-int beam_chunks(int64_t rows, int vocab, int dtype) {
-    const int vec = dtype == DLLM_DTYPE_F32 ? 4 : 8;
-    const int64_t tiles = ((int64_t)vocab + BS_NT * BS_U * vec - 1) / (BS_NT * BS_U * vec), slots = 148 * 4;
-    int best = 1;
-    int64_t least = INT64_MAX;
-    for (int c = 1; c <= tiles && c <= 64; c++) {
-        const int64_t cost = (rows * c + slots - 1) / slots * ((tiles + c - 1) / c + 2);
-        if (cost < least) {
-            least = cost;
-            best = c;
-        }
-    }
-    return best;
+// A CTA for every tile, at most as many as fit on the GPU at once.
+Split beam_split(const dllm_beam_desc *d) {
+    const int vec = d->dtype == DLLM_DTYPE_F32 ? 4 : 8;
+    Split s;
+    // rows begin anywhere in their first vector
+    if (d->mask) s.per_row = (int)((((int64_t)d->vocab + 31) / 32 + BS_NT - 1) / BS_NT);
+    else s.per_row = (int)((((int64_t)d->vocab + 2 * vec - 2) / vec + BS_NT * BS_U - 1) / (BS_NT * BS_U));
+    s.all = (int64_t)d->batch * d->beams * s.per_row;
+    const int64_t room = (int64_t)sm_count() * (d->mask ? 4 : 3);
+    s.ctas = (int)(s.all < room ? s.all : room);
+    const int64_t share = s.all / s.ctas;  // tiles of a CTA, at least
+    const int64_t most = (s.per_row + share - 2) / share + 1;
+    s.pieces = (int)(most < s.per_row ? most : s.per_row);
+    return s;
 }
 
 // ----------------------------------------------------------------------------------------
@@ -844,35 +990,33 @@ __global__ void __launch_bounds__(RO_NT) beam_reorder_kernel(ReorderArgs a) {
 }  // namespace
 
 template <auto Kernel>
-static void launch_chunks(unsigned grid, const dllm_beam_desc &d, int chunks, ChunkSum *sums, uint64_t *cands,
+static void launch_pieces(const dllm_beam_desc &d, const Split &split, PieceSum *sums, uint64_t *cands,
                           cudaStream_t stream) {
     // room for four CTAs' buffers on an SM
     set_once<Kernel>(cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-    Kernel<<<grid, BS_NT, 0, stream>>>(d, chunks, sums, cands);
+    Kernel<<<split.ctas, BS_NT, 0, stream>>>(d, split, sums, cands);
 }
 
+static size_t sums_bytes(int64_t pieces) { return ((size_t)pieces * sizeof(PieceSum) + 255) / 256 * 256; }
+
 size_t beam_ws_bytes(const dllm_beam_desc *d) {
-    const int64_t rows = (int64_t)d->batch * d->beams;
-    const size_t n = (size_t)rows * beam_chunks(rows, d->vocab, d->dtype);
-    return (n * sizeof(ChunkSum) + 255) / 256 * 256 + n * d->k * sizeof(uint64_t);
+    const int64_t n = (int64_t)d->batch * d->beams * beam_split(d).pieces;
+    return sums_bytes(n) + (size_t)n * d->k * sizeof(uint64_t);
 }
 
 dllm_status launch_beam_select(const dllm_beam_desc *d, void *ws, cudaStream_t stream) {
-    const int64_t rows = (int64_t)d->batch * d->beams;
-    const int chunks = beam_chunks(rows, d->vocab, d->dtype);
-    ChunkSum *sums = (ChunkSum *)ws;
-    uint64_t *cands = (uint64_t *)((unsigned char *)ws + ((size_t)rows * chunks * sizeof(ChunkSum) + 255) / 256 * 256);
-    if (rows * chunks > INT32_MAX) return DLLM_ERR_UNSUPPORTED;
-    const unsigned grid = (unsigned)(rows * chunks);
-#define DLLM_CHUNKS(DT)                                                                                \
-    (d->mask ? launch_chunks<beam_chunk_kernel<DT, true>>(grid, *d, chunks, sums, cands, stream)       \
-             : launch_chunks<beam_chunk_kernel<DT, false>>(grid, *d, chunks, sums, cands, stream))
-    if (d->dtype == DLLM_DTYPE_F32) DLLM_CHUNKS(DLLM_DTYPE_F32);
-    else if (d->dtype == DLLM_DTYPE_BF16) DLLM_CHUNKS(DLLM_DTYPE_BF16);
-    else DLLM_CHUNKS(DLLM_DTYPE_F16);
-#undef DLLM_CHUNKS
+    const Split split = beam_split(d);
+    PieceSum *sums = (PieceSum *)ws;
+    uint64_t *cands = (uint64_t *)((unsigned char *)ws + sums_bytes((int64_t)d->batch * d->beams * split.pieces));
+#define DLLM_PIECES(DT)                                                                       \
+    (d->mask ? launch_pieces<beam_pieces_kernel<DT, true>>(*d, split, sums, cands, stream)    \
+             : launch_pieces<beam_pieces_kernel<DT, false>>(*d, split, sums, cands, stream))
+    if (d->dtype == DLLM_DTYPE_F32) DLLM_PIECES(DLLM_DTYPE_F32);
+    else if (d->dtype == DLLM_DTYPE_BF16) DLLM_PIECES(DLLM_DTYPE_BF16);
+    else DLLM_PIECES(DLLM_DTYPE_F16);
+#undef DLLM_PIECES
     if (cudaGetLastError() != cudaSuccess) return DLLM_ERR_CUDA;
-    // launched while the chunks run; it waits for them on the GPU
+    // launched while the pieces run; it waits for them on the GPU
     cudaLaunchAttribute attr = {};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
@@ -882,7 +1026,7 @@ dllm_status launch_beam_select(const dllm_beam_desc *d, void *ws, cudaStream_t s
     cfg.stream = stream;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, beam_merge_kernel, *d, (const ChunkSum *)sums, (const uint64_t *)cands, chunks) ==
+    return cudaLaunchKernelEx(&cfg, beam_merge_kernel, *d, (const PieceSum *)sums, (const uint64_t *)cands, split) ==
                    cudaSuccess
                ? DLLM_OK
                : DLLM_ERR_CUDA;
