@@ -9,7 +9,9 @@ to a host implementation.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
+import threading
 
 import numpy as np
 
@@ -744,8 +746,8 @@ def _scratch(ws, dev):
 _torch_c = None
 
 
-def _call(name, dev, stream, *args):
-    """Runs a library call on `stream` (default: the current one of device `dev`), with `dev` current."""
+def _torch_calls():
+    """(current raw stream of a device, current device, device guard) of torch."""
     global _torch_c
     if _torch_c is None:
         import torch
@@ -753,19 +755,58 @@ def _call(name, dev, stream, *args):
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # without making a Stream object
         _torch_c = (raw or (lambda i: torch.cuda.current_stream(i).cuda_stream), torch.cuda.current_device,
                     torch.cuda.device)
-    if stream is None:
-        stream = _torch_c[0](dev)
+    return _torch_c
+
+
+def _call(name, dev, *args):
+    """Runs a library call on the current stream of device `dev`, with `dev` current."""
+    raw_stream, current, guard = _torch_calls()
     f = getattr(load_library(), name)
-    if _torch_c[1]() == dev:
-        rc = f(*args, stream)
+    if current() == dev:
+        rc = f(*args, raw_stream(dev))
     else:
-        with _torch_c[2](dev):
-            rc = f(*args, stream)
+        with guard(dev):
+            rc = f(*args, raw_stream(dev))
     if rc != DLLM_OK:
         _check(rc, name)
 
 
-def quantize_rows_i8(x, *, norm=False, norm_w=None, eps=1e-6, add_one=False, q=None, scale=None, stream=None):
+def _on_stream(function):
+    """`stream`: a raw cudaStream_t that the call runs on; what it allocates then belongs to that stream too
+    (memory of the current one could be reused there while the call still works with it)."""
+    @functools.wraps(function)
+    def on_stream(first, *args, stream=None, **kw):
+        if stream is None:
+            return function(first, *args, **kw)
+        import torch
+
+        t = first[0] if isinstance(first, (list, tuple)) and first else first
+        dev = t.device if hasattr(t, "device") else args[0].device
+        s = torch.cuda.ExternalStream(int(stream), dev) if int(stream) else torch.cuda.default_stream(dev)
+        with torch.cuda.stream(s):
+            return function(first, *args, **kw)
+    return on_stream
+
+
+_workspaces = threading.local()
+
+
+def _workspace(nbytes, device, dev):
+    """Scratch of a call on the current stream: this thread's buffer of the (device, stream), grown as
+    needed; during a stream capture a tensor of its own, which the graph's pool keeps."""
+    import torch
+
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    held, key = _workspaces.__dict__, (dev, _torch_calls()[0](dev))
+    ws = held.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = held[key] = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return ws
+
+
+@_on_stream
+def quantize_rows_i8(x, *, norm=False, norm_w=None, eps=1e-6, add_one=False, q=None, scale=None):
     """Rows to int8 codes with a scale each (dllm_cuda_quantize_rows_i8): x [rows][cols] fp32 / bf16 /
     fp16, RMS-normalised first when `norm`.  Returns (codes int8 [rows][cols], scale fp32 [rows]); the
     codes' rows start on multiples of 16 bytes."""
@@ -790,13 +831,17 @@ def quantize_rows_i8(x, *, norm=False, norm_w=None, eps=1e-6, add_one=False, q=N
             raise DllmError("q: the shape of x is needed")
     if scale is None:
         scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    _call("dllm_cuda_quantize_rows_i8", dev, stream, rows, cols, x.data_ptr(), x_stride if rows > 1 else cols, code,
+        sp = scale.data_ptr()
+    else:
+        sp = _vector(scale, rows, torch.float32, dev, "scale")
+    _call("dllm_cuda_quantize_rows_i8", dev, rows, cols, x.data_ptr(), x_stride if rows > 1 else cols, code,
           bool(norm), None if norm_w is None else _vector(norm_w, cols, torch.float32, dev, "norm_w"), eps, bool(add_one),
-          qp, ld, _vector(scale, rows, torch.float32, dev, "scale"))
+          qp, ld, sp)
     return q, scale
 
 
-def matmul_i8(a, a_scale, b, b_scale, *, softcap=0.0, out=None, out_dtype=None, status=None, stream=None):
+@_on_stream
+def matmul_i8(a, a_scale, b, b_scale, *, softcap=0.0, out=None, out_dtype=None, status=None):
     """out[i][j] = a_scale[i] b_scale[j] sum_k a[i][k] b[j][k] (dllm_cuda_matmul_i8): int8 codes a
     [m][k], b [n][k] as quantize_rows_i8 gives them, fp32 scales; out fp32 (default), bf16 or fp16."""
     import torch
@@ -819,14 +864,15 @@ def matmul_i8(a, a_scale, b, b_scale, *, softcap=0.0, out=None, out_dtype=None, 
         ldo = out.stride(0) if m > 1 else n
     if code is None:
         raise DllmError("out: fp32, bf16 or fp16 is needed")
-    _call("dllm_cuda_matmul_i8", dev, stream, m, n, k, ap, lda, _vector(a_scale, m, torch.float32, dev, "a_scale"), bp,
+    _call("dllm_cuda_matmul_i8", dev, m, n, k, ap, lda, _vector(a_scale, m, torch.float32, dev, "a_scale"), bp,
           ldb, _vector(b_scale, n, torch.float32, dev, "b_scale"), softcap, out.data_ptr(), ldo, code,
           None if status is None else _vector(status, 1, torch.int32, dev, "status"))
     return out
 
 
+@_on_stream
 def lmhead_logits_i8(h, w, w_scale, *, norm_w=None, eps=1e-6, add_one=False, softcap=0.0, logits=None, status=None,
-                     workspace=None, stream=None):
+                     workspace=None):
     """lmhead_logits with int8 output weights (dllm_cuda_lmhead_logits_i8): h fp32 [rows][hidden], w int8
     [vocab][hidden] and w_scale fp32 [vocab] from quantize_rows_i8; returns fp32 logits [rows][vocab]."""
     import torch
@@ -841,9 +887,8 @@ def lmhead_logits_i8(h, w, w_scale, *, norm_w=None, eps=1e-6, add_one=False, sof
     if logits is None:
         logits = torch.empty((rows, vocab), dtype=torch.float32, device=h.device)
     if workspace is None:
-        workspace = torch.empty(load_library().dllm_cuda_lmhead_i8_workspace_bytes(rows, hidden), dtype=torch.uint8,
-                                device=h.device)
-    _call("dllm_cuda_lmhead_logits_i8", dev, stream, rows, hidden, vocab, h.data_ptr(),
+        workspace = _workspace(load_library().dllm_cuda_lmhead_i8_workspace_bytes(rows, hidden), h.device, dev)
+    _call("dllm_cuda_lmhead_logits_i8", dev, rows, hidden, vocab, h.data_ptr(),
           None if norm_w is None else _vector(norm_w, hidden, torch.float32, dev, "norm_w"), eps, bool(add_one), wp, ldw,
           _vector(w_scale, vocab, torch.float32, dev, "w_scale"), softcap,
           _vector(logits, rows * vocab, torch.float32, dev, "logits"),
@@ -855,7 +900,8 @@ def lmhead_logits_i8(h, w, w_scale, *, norm_w=None, eps=1e-6, add_one=False, sof
 
 def fill_beam_desc(logits, scores, k, *, mask=None, finished=None, eos=-1, lengths=None, length_penalty=0.0, out=None,
                    out_finished=None, out_lengths=None, status=None, workspace=None):
-    """Builds a dllm_beam_desc from CUDA tensors; returns (desc, (score, parent, token), workspace)."""
+    """Builds a dllm_beam_desc from CUDA tensors; returns (desc, (score, parent, token)).  The workspace is
+    left out where none is given."""
     import torch
 
     code, dev = _float_code(logits.dtype), logits.get_device()
@@ -880,35 +926,46 @@ def fill_beam_desc(logits, scores, k, *, mask=None, finished=None, eos=-1, lengt
             raise DllmError(f"mask: int32 words [{rows}][{words}] on cuda:{dev} are needed")
         mask_ptr, mask_stride = mask.data_ptr(), mask.stride(0) if rows > 1 else words
     if out is None:
-        score, parent, token = torch.empty((3, batch, max(k, 0)), dtype=torch.int32, device=logits.device).unbind(0)
-        score = score.view(torch.float32)
-        out = (score, parent, token)
+        buf = torch.empty((3, batch, max(k, 0)), dtype=torch.int32, device=logits.device)
+        score, parent, token = buf.unbind(0)
+        out = (score.view(torch.float32), parent, token)
+        p = buf.data_ptr()
+        out_ptrs = (p, p + 4 * n, p + 8 * n)
     else:
         score, parent, token = out
+        out_ptrs = (_vector(score, n, torch.float32, dev, "out score"), _vector(parent, n, torch.int32, dev, "out parent"),
+                    _vector(token, n, torch.int32, dev, "out token"))
     d = BeamDesc(batch, beams, vocab, k, row_stride if rows > 1 else vocab, code, logits.data_ptr(), mask_ptr, mask_stride,
                  _vector(scores, rows, torch.float32, dev, "scores"),
                  None if finished is None else _flags(finished, rows, dev, "finished"), int(eos),
                  None if lengths is None else _vector(lengths, rows, torch.int32, dev, "lengths"), length_penalty,
-                 _vector(score, n, torch.float32, dev, "out score"), _vector(parent, n, torch.int32, dev, "out parent"),
-                 _vector(token, n, torch.int32, dev, "out token"),
+                 *out_ptrs,
                  None if out_finished is None else _flags(out_finished, n, dev, "out_finished"),
                  None if out_lengths is None else _vector(out_lengths, n, torch.int32, dev, "out_lengths"),
                  None if status is None else _vector(status, rows, torch.int32, dev, "status"))
-    if workspace is None:
-        workspace = torch.empty(load_library().dllm_cuda_beam_workspace_bytes(C.byref(d)), dtype=torch.uint8,
-                                device=logits.device)
-    d.workspace, d.workspace_bytes = _scratch(workspace, dev)
-    return d, out, workspace
+    if workspace is not None:
+        d.workspace, d.workspace_bytes = _scratch(workspace, dev)
+    return d, out
 
 
-def beam_select(logits, scores, k, *, stream=None, **kw):
+def beam_workspace_bytes(logits, scores, k, **kw) -> int:
+    """dllm_cuda_beam_workspace_bytes for the same arguments as beam_select."""
+    return int(load_library().dllm_cuda_beam_workspace_bytes(C.byref(fill_beam_desc(logits, scores, k, **kw)[0])))
+
+
+@_on_stream
+def beam_select(logits, scores, k, **kw):
     """The k best continuations of each sequence's beams (dllm_cuda_beam_select): logits [batch * beams]
     [vocab], scores fp32 [batch][beams].  Returns (score fp32, parent int32, token int32), each
     [batch][k], best rank first; a slot that nothing fills has (-inf, -1, -1).  Options: `mask`
     (packed allow-bits), `finished` and `eos` (ended beams), `lengths` and `length_penalty`, `out`
     (the three outputs), `out_finished`, `out_lengths`, `status`, `workspace`."""
-    d, out, ws = fill_beam_desc(logits, scores, k, **kw)
-    _call("dllm_cuda_beam_select", logits.get_device(), stream, C.byref(d))
+    d, out = fill_beam_desc(logits, scores, k, **kw)
+    dev, p = logits.get_device(), C.byref(d)
+    if not d.workspace:
+        ws = _workspace(load_library().dllm_cuda_beam_workspace_bytes(p), logits.device, dev)
+        d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
+    _call("dllm_cuda_beam_select", dev, p)
     return out
 
 
@@ -932,7 +989,8 @@ def _runs(t):
     return strides[0] * esz, segs, seg_stride, run
 
 
-def beam_reorder(states, parents, *, stream=None):
+@_on_stream
+def beam_reorder(states, parents):
     """Moves states after their beams' parents, in place (dllm_cuda_beam_reorder): every tensor of
     `states` [batch * beams][...] gets row (s, b) from row (s, parents[s][b]); parents int32
     [batch][beams], -1 leaves the beam as it is.  A view, such as the used part of a cache, is moved
@@ -955,5 +1013,5 @@ def beam_reorder(states, parents, *, stream=None):
             seen.add(ptr)
             groups.setdefault(_runs(t), []).append(ptr)
     for (row, segs, seg, run), ptrs in groups.items():
-        _call("dllm_cuda_beam_reorder", dev, stream, batch, beams, parents.data_ptr(), len(ptrs),
+        _call("dllm_cuda_beam_reorder", dev, batch, beams, parents.data_ptr(), len(ptrs),
               (C.c_void_p * len(ptrs))(*ptrs), row, segs, seg, run)

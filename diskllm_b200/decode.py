@@ -123,7 +123,10 @@ class BeamLoop:
         self.logits = buf(rows, wq.shape[0], dtype=torch.float32)
         self.head_ws = buf(max(1, capi.load_library().dllm_cuda_lmhead_i8_workspace_bytes(rows, wq.shape[1])),
                            dtype=torch.uint8)
-        _, _, self.beam_ws = capi.fill_beam_desc(self.logits, self.scores, beams, eos=eos)
+        self.beam_ws = buf(capi.beam_workspace_bytes(self.logits, self.scores, beams), dtype=torch.uint8)
+        if mask_ring is not None:  # rows with a mask are dealt out differently
+            masked = capi.beam_workspace_bytes(self.logits, self.scores, beams, mask=mask_ring[0])
+            self.beam_ws = buf(max(masked, self.beam_ws.numel()), dtype=torch.uint8)
         self.graph = None
 
     @property

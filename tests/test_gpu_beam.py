@@ -311,8 +311,8 @@ def test_select_capture_without_a_workspace_is_refused():
     import ctypes as C
 
     x, sc = torch.zeros(4, 100, device=DEV), torch.zeros(1, 4, device=DEV)
-    d, out, _ = capi.fill_beam_desc(x, sc, 4)
-    d.workspace, d.workspace_bytes = None, 0
+    d, out = capi.fill_beam_desc(x, sc, 4)
+    assert not d.workspace
     g = torch.cuda.CUDAGraph()
     torch.cuda.synchronize()
     with torch.cuda.graph(g):
@@ -464,3 +464,76 @@ def test_reorder_refusals():
         with pytest.raises(capi.DllmError):
             call()
     assert (t == 0).all()
+
+
+# ---- how the calls share memory --------------------------------------------------------------
+
+def test_captured_calls_keep_their_scratch():
+    """graphs captured without a workspace have scratch of their own: larger eager calls in between, which
+    grow the eager scratch, and two graphs replayed at once on two streams do not disturb them"""
+    rng = np.random.default_rng(31)
+    xs = [rows(rng, 8, 30000, torch.float32) for _ in range(2)]
+    sc = beam_scores(rng, 2, 4)
+    want = [[t.clone() for t in capi.beam_select(x, sc, 8)] for x in xs]
+    graphs, outs = [], []
+    torch.cuda.synchronize()
+    for x in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(capi.beam_select(x, sc, 8))
+        graphs.append(g)
+    big = rows(rng, 64, 50000, torch.float32)
+    capi.beam_select(big, beam_scores(rng, 8, 8), 64)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert all(torch.equal(a, b) for a, b in zip(o, w))
+
+
+def test_stream_argument():
+    rng = np.random.default_rng(32)
+    x, sc = rows(rng, 8, 30000, torch.float32), beam_scores(rng, 2, 4)
+    want = capi.beam_select(x, sc, 4)
+    t = torch.randn(8, 100, device=DEV)
+    after = moved(t, want[1])
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = capi.beam_select(x, sc, 4, stream=s.cuda_stream)
+    capi.beam_reorder([t], got[1], stream=s.cuda_stream)
+    q, scale = capi.quantize_rows_i8(t, stream=s.cuda_stream)
+    m = capi.matmul_i8(q, scale, q, scale, stream=s.cuda_stream)
+    lg = capi.lmhead_logits_i8(t, q, scale, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(t, after)
+    q2, scale2 = capi.quantize_rows_i8(t)
+    assert torch.equal(q, q2) and torch.equal(m, capi.matmul_i8(q2, scale2, q2, scale2))
+    assert torch.equal(lg, capi.lmhead_logits_i8(t, q2, scale2))
+    assert torch.equal(capi.beam_select(x, sc, 4, stream=0)[2], want[2])
+
+
+def test_calls_from_several_threads():
+    import threading
+
+    rng = np.random.default_rng(33)
+    cases = [(rows(rng, 4 * n, 9000 * n, torch.float32), beam_scores(rng, n, 4)) for n in (1, 2, 3, 5)]
+    want = [capi.beam_select(x, sc, 6) for x, sc in cases]
+    bad = []
+
+    def go(i):
+        for _ in range(30):
+            got = capi.beam_select(*cases[i], 6)
+            torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                bad.append(i)
+
+    threads = [threading.Thread(target=go, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad

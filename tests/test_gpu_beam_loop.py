@@ -55,8 +55,9 @@ def test_every_step(batch, beams, masked, alpha):
         assert torch.equal(bl.hist[:, :i + 1], hist)
 
 
-def test_graph_replay_equals_eager():
-    bl, _ = loop(np.random.default_rng(4), 2, 4, 8, length_penalty=0.6)
+@pytest.mark.parametrize("masked", [False, True])
+def test_graph_replay_equals_eager(masked):
+    bl, _ = loop(np.random.default_rng(4), 2, 4, 8, length_penalty=0.6, masked=masked)
     start = [t.clone() for t in bl.states]
     want = bl.run_eager().clone()
     results = [t.clone() for t in (bl.scores, bl.lengths, bl.finished, *bl.states)]
