@@ -386,6 +386,58 @@ __device__ __forceinline__ float tanh_above_one(float z) {
     return copysignf(__fmaf_rn(-2.0f, r, 1.0f), z);
 }
 
+// Half of a tile's 16-column groups: the warp's 32 channels, from its lanes' accumulators, scaled, capped
+// and stored.
+template <int DT, bool CAP>
+__device__ __forceinline__ void store_tile(const MmArgs &p, uint32_t lanes, int half, int ch, int t0, const float *sa,
+                               float sb) {
+    for (int c = half * 16; c < p.nt; c += 32) {
+        int r[16];
+        __syncwarp();
+        tmem_load16(lanes + c, r);
+        float v[16];
+        float big = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+            const float4 s4 = *(const float4 *)(sa + c + j);
+            Pair lo = mul2(mul2(Pair((float)r[j], (float)r[j + 1]), Pair(s4.x, s4.y)), Pair(sb, sb));
+            Pair hi = mul2(mul2(Pair((float)r[j + 2], (float)r[j + 3]), Pair(s4.z, s4.w)), Pair(sb, sb));
+            if (CAP) {
+                float z[4];
+                lo.split(z[0], z[1]);
+                hi.split(z[2], z[3]);
+                lo = tanh2(lo);
+                hi = tanh2(hi);
+                big = fmaxf(fmaxf(fabsf(z[0]), fabsf(z[1])), fmaxf(fabsf(z[2]), fabsf(z[3])));
+                if (__any_sync(0xffffffffu, big > 1.0f)) {
+                    float y[4];
+                    lo.split(y[0], y[1]);
+                    hi.split(y[2], y[3]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (fabsf(z[i]) > 1.0f) y[i] = tanh_above_one(z[i]);
+                    lo = Pair(y[0], y[1]);
+                    hi = Pair(y[2], y[3]);
+                }
+                lo = mul2(lo, Pair(p.softcap, p.softcap));
+                hi = mul2(hi, Pair(p.softcap, p.softcap));
+            }
+            lo.split(v[j], v[j + 1]);
+            hi.split(v[j + 2], v[j + 3]);
+        }
+        if (ch >= p.n) continue;
+        int64_t at = (int64_t)(t0 + c) * p.ldo + ch;
+        if (t0 + c + 16 <= p.m) {
+#pragma unroll
+            for (int j = 0; j < 16; j++, at += p.ldo) store_out<DT>(p.out, at, v[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; j++, at += p.ldo)
+                if (t0 + c + j < p.m) store_out<DT>(p.out, at, v[j]);
+        }
+    }
+}
+
 // Persistent, one CTA per SM.  Warp 0 copies tiles (TMA), warp 1 issues the products, warps 2 to 9
 // scale and store; two accumulators, so that a tile's stores run under the next tile's products.
 template <int DT, bool CAP>
@@ -472,10 +524,11 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_kernel(const __grid_c
                 load_b();
                 load_a();
             }
-            // no copy may be in flight when the CTA ends, also where a wait ran out
+            // no copy may be in flight when the CTA ends, also where a wait ran out, nor a product's arrival
             volatile int alone = 0;
+            const uint32_t last = gave_up ? full : empty;
             for (uint32_t i = step < (uint32_t)p.stages ? 0 : step - p.stages; i < step; i++)
-                mbar_wait(full + 8 * (i % p.stages), (i / p.stages) & 1, &alone);
+                mbar_wait(last + 8 * (i % p.stages), (i / p.stages) & 1, &alone);
         }
         __syncwarp();
     } else if (wid == 1) {
@@ -525,50 +578,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_kernel(const __grid_c
             int ok = mbar_wait(done + 8 * acc, (it >> 1) & 1, &gave_up);
             if (!__all_sync(0xffffffffu, ok)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            for (int c = half * 16; c < p.nt; c += 32) {
-                int r[16];
-                tmem_load16(tmem + acc * p.nt + c + ((uint32_t)quarter << 21), r);
-                float v[16];
-                float big = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 16; j += 4) {
-                    const float4 s4 = *(const float4 *)(sa + c + j);
-                    Pair lo = mul2(mul2(Pair((float)r[j], (float)r[j + 1]), Pair(s4.x, s4.y)), Pair(sb, sb));
-                    Pair hi = mul2(mul2(Pair((float)r[j + 2], (float)r[j + 3]), Pair(s4.z, s4.w)), Pair(sb, sb));
-                    if (CAP) {
-                        float z[4];
-                        lo.split(z[0], z[1]);
-                        hi.split(z[2], z[3]);
-                        lo = tanh2(lo);
-                        hi = tanh2(hi);
-                        big = fmaxf(fmaxf(fabsf(z[0]), fabsf(z[1])), fmaxf(fabsf(z[2]), fabsf(z[3])));
-                        if (__any_sync(0xffffffffu, big > 1.0f)) {
-                            float y[4];
-                            lo.split(y[0], y[1]);
-                            hi.split(y[2], y[3]);
-#pragma unroll
-                            for (int i = 0; i < 4; i++)
-                                if (fabsf(z[i]) > 1.0f) y[i] = tanh_above_one(z[i]);
-                            lo = Pair(y[0], y[1]);
-                            hi = Pair(y[2], y[3]);
-                        }
-                        lo = mul2(lo, Pair(p.softcap, p.softcap));
-                        hi = mul2(hi, Pair(p.softcap, p.softcap));
-                    }
-                    lo.split(v[j], v[j + 1]);
-                    hi.split(v[j + 2], v[j + 3]);
-                }
-                if (ch >= p.n) continue;
-                int64_t at = (int64_t)(t0 + c) * p.ldo + ch;
-                if (t0 + c + 16 <= p.m) {
-#pragma unroll
-                    for (int j = 0; j < 16; j++, at += p.ldo) store_out<DT>(p.out, at, v[j]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 16; j++, at += p.ldo)
-                        if (t0 + c + j < p.m) store_out<DT>(p.out, at, v[j]);
-                }
-            }
+            store_tile<DT, CAP>(p, tmem + acc * p.nt + ((uint32_t)quarter << 21), half, ch, t0, sa, sb);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(drained + 8 * acc);
@@ -647,8 +657,9 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_split_kernel(const __
                 load_a(i);
             }
             volatile int alone = 0;
+            const uint32_t last = gave_up ? full : empty;
             for (int j = i < p.stages ? 0 : i - p.stages; j < i; j++)
-                mbar_wait(full + 8 * (j % p.stages), (j / p.stages) & 1, &alone);
+                mbar_wait(last + 8 * (j % p.stages), (j / p.stages) & 1, &alone);
         }
         __syncwarp();
     } else if (wid == 1) {
@@ -819,20 +830,21 @@ dllm_status launch_matmul_i8(int m, int n, int k, const int8_t *a, int64_t lda, 
     // token tiles of equal size, at most 256 (the widest instruction)
     p.token_tiles = (m + 255) / 256;
     p.nt = ((m + p.token_tiles - 1) / p.token_tiles + 15) / 16 * 16;
+    const int sms = sm_count(), kblocks = (k + MM_KB - 1) / MM_KB;
+    const int64_t tiles = (int64_t)((n + MM_ROWS - 1) / MM_ROWS) * p.token_tiles;
+    // few tiles: split k over a cluster of up to 8 CTAs, while the SMs suffice and a part has 4 blocks
+    int parts = 1;
+    while (parts < 8 && tiles * parts * 2 <= sms && kblocks >= parts * 8) parts *= 2;
     p.stages = (MM_SMEM - 1024) / ((MM_ROWS + p.nt) * MM_KB);
     if (p.stages > MM_MAX_STAGES) p.stages = MM_MAX_STAGES;
     p.tmem_cols = 32;
     while (p.tmem_cols < 2 * p.nt) p.tmem_cols *= 2;
     CUtensorMap map_a, map_b;
-    if (!code_map(&map_a, a, m, k, lda, p.nt) || !code_map(&map_b, b, n, k, ldb, MM_ROWS)) return DLLM_ERR_CUDA;
-    const int64_t tiles = (int64_t)((n + MM_ROWS - 1) / MM_ROWS) * p.token_tiles;
-    const int sms = sm_count(), kblocks = (k + MM_KB - 1) / MM_KB;
-    // few tiles: split k over a cluster of up to 8 CTAs, while the SMs suffice and a part has 4 blocks
-    int parts = 1;
-    while (parts < 8 && tiles * parts * 2 <= sms && kblocks >= parts * 8) parts *= 2;
+    if (!code_map(&map_a, a, m, k, lda, p.nt) || !code_map(&map_b, b, n, k, ldb, MM_ROWS))
+        return DLLM_ERR_CUDA;
     cudaLaunchAttribute attr[2] = {};
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(parts > 1 ? (unsigned)(tiles * parts) : (unsigned)(tiles < sms ? tiles : sms));
+    cfg.gridDim = dim3((unsigned)(parts > 1 ? tiles * parts : tiles < sms ? tiles : sms));
     cfg.blockDim = dim3(MM_THREADS);
     cfg.dynamicSmemBytes = MM_SMEM;
     cfg.stream = stream;

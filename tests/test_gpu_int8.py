@@ -126,7 +126,9 @@ def test_quantize_no_rows():
 
 SIZES = [(1, 1, 1), (1, 130, 16), (2, 127, 100), (5, 257, 33), (8, 128, 128), (16, 1000, 129), (17, 300, 640),
          (31, 64, 2304), (33, 129, 255), (64, 512, 4096), (100, 333, 1000), (128, 200, 512), (129, 100, 96),
-         (200, 384, 1030), (256, 256, 384), (257, 131, 70), (300, 1111, 600), (513, 520, 200), (3, 20000, 64)]
+         (200, 384, 1030), (256, 256, 384), (257, 131, 70), (300, 1111, 600), (513, 520, 200), (3, 20000, 64),
+         # several tiles for every SM, whole and ragged in both directions, short and long k
+         (512, 19000, 160), (400, 25025, 33), (1001, 9999, 300), (2048, 4736, 96), (3001, 4097, 640), (700, 13000, 2050)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
