@@ -250,6 +250,13 @@ __device__ __forceinline__ float load_one(const void *row, int i) {
     return DT == DLLM_DTYPE_BF16 ? __uint_as_float((uint32_t)u << 16) : __half2float(__ushort_as_half(u));
 }
 
+template <int DT>
+__device__ __forceinline__ float load_shared(const void *elems, int i) {
+    if (DT == DLLM_DTYPE_F32) return ((const float *)elems)[i];
+    const unsigned short u = ((const unsigned short *)elems)[i];
+    return DT == DLLM_DTYPE_BF16 ? __uint_as_float((uint32_t)u << 16) : __half2float(__ushort_as_half(u));
+}
+
 // A warp sorts its candidates, best first; the k-th.
 __device__ __noinline__ uint64_t warp_sorts(uint64_t *mine, int count, int k) {
     const int lane = threadIdx.x & 31;
@@ -264,6 +271,7 @@ struct PieceShared {
     uint64_t buf[BS_CAP];          // [warp][BS_WCAP] candidates
     uint64_t few[BS_NT];
     Tops tops;
+    uint4 held[BS_WARPS][BS_U];    // the vectors of a lane that holds a candidate
     uint32_t floor_key;
     int wcount[BS_WARPS];
     float wm[BS_WARPS];
@@ -496,23 +504,6 @@ __device__ __forceinline__ void dense_piece(const dllm_beam_desc &d, PieceShared
         c.s += (double)part.sum();
         return tm;
     };
-    // the warp looks at one lane's vector together, an element in each lane
-    auto offer_vector = [&](const uint4 &v, int holder, int j) {
-        const int e = c.lane % VEC;
-        const uint4 o = make_uint4(__shfl_sync(0xffffffffu, v.x, holder), __shfl_sync(0xffffffffu, v.y, holder),
-                                   __shfl_sync(0xffffffffu, v.z, holder), __shfl_sync(0xffffffffu, v.w, holder));
-        float f;
-        if (DT == DLLM_DTYPE_F32) f = __uint_as_float(word_of(o, e));
-        else {
-            const float2 pr = pair_of<DT>(make_uint4(word_of(o, e / 2), 0, 0, 0), 0);
-            f = e & 1 ? pr.y : pr.x;
-        }
-        c.offer(c.lane < VEC, f, j * VEC - shift + e);
-    };
-    auto holders_of = [&](const uint4 &v) {
-        const uint4 one[1] = {v};
-        return __ballot_sync(0xffffffffu, largest<DT, 1>(one) >= okey_value(c.thr));
-    };
     for (int t0 = v0;;) {
 #pragma unroll
         for (int u = 0; u < BS_U; u++) x[u] = next[u];
@@ -521,11 +512,18 @@ __device__ __forceinline__ void dense_piece(const dllm_beam_desc &d, PieceShared
         c.tile++;
         if (c.tile == 1) c.settle_threshold();  // with every warp's first tile
         else c.raise_threshold();
-        if (__any_sync(0xffffffffu, tm >= okey_value(c.thr)))
+        // Lanes that hold a candidate are rare: each puts its vectors into shared memory, where the warp
+        // looks at them together, an element in each lane.
+        for (uint32_t who = __ballot_sync(0xffffffffu, tm >= okey_value(c.thr)); who; who &= who - 1) {
+            const int holder = __ffs(who) - 1, e = c.lane % (BS_U * VEC);
+            if (c.lane == holder)
 #pragma unroll
-            for (int u = 0; u < BS_U; u++)
-                for (uint32_t hit = holders_of(x[u]); hit; hit &= hit - 1)
-                    offer_vector(x[u], __ffs(hit) - 1, t0 + u * BS_NT + c.wid * 32 + __ffs(hit) - 1);
+                for (int u = 0; u < BS_U; u++) sh.held[c.wid][u] = x[u];
+            __syncwarp();
+            const float f = load_shared<DT>(sh.held[c.wid], e);
+            c.offer(c.lane < BS_U * VEC, f, (t0 + e / VEC * BS_NT + c.wid * 32 + holder) * VEC - shift + e % VEC);
+            __syncwarp();
+        }
         t0 += TILE;
         if (t0 >= v1) break;
     }
