@@ -775,16 +775,15 @@ def _on_stream(function):
     """`stream`: a raw cudaStream_t that the call runs on; what it allocates then belongs to that stream too
     (memory of the current one could be reused there while the call still works with it)."""
     @functools.wraps(function)
-    def on_stream(first, *args, stream=None, **kw):
+    def on_stream(*args, stream=None, **kw):
         if stream is None:
-            return function(first, *args, **kw)
+            return function(*args, **kw)
         import torch
 
-        t = first[0] if isinstance(first, (list, tuple)) and first else first
-        dev = t.device if hasattr(t, "device") else args[0].device
+        dev = next(t.device for t in (*args, *kw.values()) if isinstance(t, torch.Tensor))
         s = torch.cuda.ExternalStream(int(stream), dev) if int(stream) else torch.cuda.default_stream(dev)
         with torch.cuda.stream(s):
-            return function(first, *args, **kw)
+            return function(*args, **kw)
     return on_stream
 
 
@@ -821,7 +820,7 @@ def quantize_rows_i8(x, *, norm=False, norm_w=None, eps=1e-6, add_one=False, q=N
         raise DllmError("x: contiguous rows of at least one element are needed")
     if q is None:
         ld = (cols + 15) // 16 * 16
-        q = torch.empty((rows, ld), dtype=torch.int8, device=x.device)
+        q = x.new_empty((rows, ld), dtype=torch.int8)
         qp = q.data_ptr()
         if ld != cols:
             q = q[:, :cols]
@@ -830,7 +829,7 @@ def quantize_rows_i8(x, *, norm=False, norm_w=None, eps=1e-6, add_one=False, q=N
         if (qr, qc) != (rows, cols):
             raise DllmError("q: the shape of x is needed")
     if scale is None:
-        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+        scale = x.new_empty(rows, dtype=torch.float32)
         sp = scale.data_ptr()
     else:
         sp = _vector(scale, rows, torch.float32, dev, "scale")
@@ -854,7 +853,7 @@ def matmul_i8(a, a_scale, b, b_scale, *, softcap=0.0, out=None, out_dtype=None, 
     if k != kb:
         raise DllmError(f"a has {k} columns, b {kb}")
     if out is None:
-        out = torch.empty((m, n), dtype=out_dtype or torch.float32, device=a.device)
+        out = a.new_empty((m, n), dtype=out_dtype or torch.float32)
         code, ldo = _float_code(out.dtype), n
     else:
         code = _float_code(out.dtype)
@@ -885,7 +884,7 @@ def lmhead_logits_i8(h, w, w_scale, *, norm_w=None, eps=1e-6, add_one=False, sof
     if hidden != hw:
         raise DllmError(f"h has {hidden} columns, w {hw}")
     if logits is None:
-        logits = torch.empty((rows, vocab), dtype=torch.float32, device=h.device)
+        logits = h.new_empty((rows, vocab))
     if workspace is None:
         workspace = _workspace(load_library().dllm_cuda_lmhead_i8_workspace_bytes(rows, hidden), h.device, dev)
     _call("dllm_cuda_lmhead_logits_i8", dev, rows, hidden, vocab, h.data_ptr(),
@@ -926,7 +925,7 @@ def fill_beam_desc(logits, scores, k, *, mask=None, finished=None, eos=-1, lengt
             raise DllmError(f"mask: int32 words [{rows}][{words}] on cuda:{dev} are needed")
         mask_ptr, mask_stride = mask.data_ptr(), mask.stride(0) if rows > 1 else words
     if out is None:
-        buf = torch.empty((3, batch, max(k, 0)), dtype=torch.int32, device=logits.device)
+        buf = logits.new_empty((3, batch, max(k, 0)), dtype=torch.int32)
         score, parent, token = buf.unbind(0)
         out = (score.view(torch.float32), parent, token)
         p = buf.data_ptr()

@@ -679,7 +679,10 @@ constexpr int BM_HELD = 4;  // candidates that a thread keeps in registers
 __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, const PieceSum *sums,
                                                            const uint64_t *cands, Split split) {
     __shared__ int npieces[DLLM_BEAM_MAX];
-    __shared__ double lse[DLLM_BEAM_MAX], inv_len[DLLM_BEAM_MAX];
+    // log-sum-exp of a row: its maximum, and what is added to that (the sum of both would lose it where
+    // logits are huge)
+    __shared__ float row_max[DLLM_BEAM_MAX];
+    __shared__ double log_sum[DLLM_BEAM_MAX], inv_len[DLLM_BEAM_MAX];
     __shared__ float score_in[DLLM_BEAM_MAX];  // copies, so that the outputs may lie over the inputs
     __shared__ int length_in[DLLM_BEAM_MAX];
     __shared__ int live[DLLM_BEAM_MAX];  // 0 nothing to offer, 1 its row's continuations, 2 ended
@@ -704,7 +707,10 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
         npieces[b] = split.cta_of((row + 1) * split.per_row - 1) - split.cta_of(row * split.per_row) + 1;
         length_in[b] = len_in;
         score_in[b] = sc;
-        inv_len[b] = d.length_penalty != 0.0f && d.lengths ? 1.0 / pow(len, (double)d.length_penalty) : 1.0;
+        // kept within 1e-200 and 1e200, so that ranks stay finite
+        inv_len[b] = d.length_penalty != 0.0f && d.lengths
+                         ? fmin(fmax(pow(len, -(double)d.length_penalty), 1e-200), 1e200)
+                         : 1.0;
         live[b] = !(sc >= -FLT_MAX && sc <= FLT_MAX) ? 0 : ended ? 2 : 1;
     }
     __syncthreads();
@@ -727,10 +733,10 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
     for (int b = wid; b < K; b += BS_WARPS) {
         const int64_t row = item * K + b;
         int st = 0, kind = live[b];
+        float M = -INFINITY;
         double l = 0.0;
         if (kind == 0 && !(score_in[b] < 0.0f)) st = DLLM_ROW_ERR_NONFINITE;  // NaN or +inf
         if (kind == 1) {
-            float M = -INFINITY;
             double S = 0.0;
             const PieceSum *mysums = sums + row * lists;
             if (npieces[b] <= 32) {
@@ -750,17 +756,21 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
             if (S != S || M == INFINITY) {
                 st = DLLM_ROW_ERR_NONFINITE;
                 kind = 0;
-            } else if (M > -INFINITY) l = (sum_base(M) + log2(S)) * (1.0 / (double)LOG2E);
+            } else if (M > -INFINITY) l = (log2(S) + (sum_base(M) - (double)M * (double)LOG2E)) * (1.0 / (double)LOG2E);
             else kind = 0;
         }
         __syncwarp();
         if (lane == 0) {
-            lse[b] = l;
+            row_max[b] = M;
+            log_sum[b] = l;
             live[b] = kind;
             if (d.status) d.status[row] = st;
         }
     }
     __syncthreads();
+    auto log_prob = [&](int b, uint64_t comp) {
+        return ((double)okey_value((uint32_t)(comp >> 32)) - (double)row_max[b]) - log_sum[b];
+    };
     // candidate e: position e % k of a piece's list; an ended beam offers its first position only
     auto candidate_of = [&](int e, int b, uint64_t comp, Best *c) {
         double cum = (double)score_in[b];
@@ -770,7 +780,7 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
             comp = composite(0, d.eos);
         } else {
             if (!comp) return false;
-            cum += (double)okey_value((uint32_t)(comp >> 32)) - lse[b];
+            cum += log_prob(b, comp);
         }
         *c = {cum * inv_len[b], b, comp};
         return true;
@@ -783,7 +793,7 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
         float score = -INFINITY;
         if (!none) {
             double cum = (double)score_in[c.beam];
-            if (live[c.beam] == 1) cum += (double)okey_value((uint32_t)(c.comp >> 32)) - lse[c.beam];
+            if (live[c.beam] == 1) cum += log_prob(c.beam, c.comp);
             score = __double2float_rn(cum);
         }
         d.out_score[item * k + place] = score;
@@ -962,12 +972,14 @@ __global__ void __launch_bounds__(RO_NT) beam_reorder_kernel(ReorderArgs a) {
     __syncthreads();
     const int64_t col = ((int64_t)slice * blockDim.x + tid) * VB;
     if (col >= a.run) return;
+    const int tail = a.run - col < VB ? (int)(a.run - col) : 0;  // bytes of a run's last, shorter vector
     unsigned char *base = a.tensors[tensor] + item * K * a.row_stride + seg * a.seg_stride + col;
     unsigned char *mine = stage + (size_t)tid * VB;
     const size_t pitch = (size_t)blockDim.x * VB;
     for (int p = 0; p < K; p++) {
         if (!needed[p]) continue;
         if (VB == 1) mine[p * pitch] = base[p * a.row_stride];
+        else if (tail) for (int i = 0; i < tail; i++) mine[p * pitch + i] = base[p * a.row_stride + i];
         else {
             const uint32_t to = (uint32_t)__cvta_generic_to_shared(mine + p * pitch);
             asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(base + p * a.row_stride), "n"(VB < 4 ? 4 : VB)
@@ -979,7 +991,8 @@ __global__ void __launch_bounds__(RO_NT) beam_reorder_kernel(ReorderArgs a) {
         if (from[j] < 0) continue;
         const unsigned char *src = mine + from[j] * pitch;
         unsigned char *dst = base + j * a.row_stride;
-        if (VB == 16) *(uint4 *)dst = *(const uint4 *)src;
+        if (VB > 1 && tail) for (int i = 0; i < tail; i++) dst[i] = src[i];
+        else if (VB == 16) *(uint4 *)dst = *(const uint4 *)src;
         else if (VB == 4) *(uint32_t *)dst = *(const uint32_t *)src;
         else *dst = *src;
     }
@@ -1032,7 +1045,8 @@ dllm_status launch_beam_select(const dllm_beam_desc *d, void *ws, cudaStream_t s
 
 dllm_status launch_beam_reorder(int batch, int beams, const int32_t *parent, int ntensors, void *const *tensors,
                                 int64_t row_stride, int segs, int64_t seg_stride, int64_t run, cudaStream_t stream) {
-    uintptr_t bits = (uintptr_t)row_stride | (uintptr_t)run | (segs > 1 ? (uintptr_t)seg_stride : 0);
+    // the widest vectors that every run's start allows
+    uintptr_t bits = (uintptr_t)row_stride | (segs > 1 ? (uintptr_t)seg_stride : 0);
     for (int i = 0; i < ntensors; i++) bits |= (uintptr_t)tensors[i];
     const int vb = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
     ReorderArgs a = {};
@@ -1044,7 +1058,7 @@ dllm_status launch_beam_reorder(int batch, int beams, const int32_t *parent, int
     a.seg_stride = seg_stride;
     a.run = run;
     const int nt = beams <= 32 ? RO_NT : 64;
-    const int64_t slices = (run / vb + nt - 1) / nt, per_tensor = slices * segs * batch;
+    const int64_t slices = ((run + vb - 1) / vb + nt - 1) / nt, per_tensor = slices * segs * batch;
     if (slices > INT32_MAX || slices * segs > INT32_MAX || per_tensor > INT32_MAX) return DLLM_ERR_UNSUPPORTED;
     a.slices = (int)slices;
     const int group = (int)(INT32_MAX / per_tensor < RO_TENSORS ? INT32_MAX / per_tensor : RO_TENSORS);

@@ -367,6 +367,10 @@ static dllm_status check_beam(const dllm_beam_desc *d) {
         set_last_error_message("more than 128 beams or 256 continuations");
         return DLLM_ERR_UNSUPPORTED;
     }
+    if (d->vocab > (1 << 30)) {
+        set_last_error_message("more than 2^30 ids");
+        return DLLM_ERR_UNSUPPORTED;
+    }
     if (d->row_stride < d->vocab) return invalid("row_stride < vocab");
     if (d->mask && d->mask_stride < ((int64_t)d->vocab + 31) / 32) return invalid("mask_stride is too small");
     if (!(d->length_penalty >= -3.4e38f && d->length_penalty <= 3.4e38f)) return invalid("length_penalty is not finite");
@@ -381,7 +385,7 @@ static dllm_status check_beam(const dllm_beam_desc *d) {
 
 extern "C" size_t dllm_cuda_beam_workspace_bytes(const dllm_beam_desc *d) {
     if (!d || d->batch < 1 || d->beams < 1 || d->vocab < 1 || d->k < 1 || d->beams > DLLM_BEAM_MAX ||
-        d->k > DLLM_BEAM_K_MAX || !float_dtype(d->dtype))
+        d->k > DLLM_BEAM_K_MAX || d->vocab > (1 << 30) || !float_dtype(d->dtype))
         return 0;
     return beam_ws_bytes(d);
 }
@@ -416,6 +420,7 @@ extern "C" dllm_status dllm_cuda_beam_reorder(int batch, int beams, const int32_
     if (!fits) return invalid("runs of a state overlap");
     for (int i = 0; i < ntensors; i++) {
         if (!tensors[i]) return invalid("a state is NULL");
+        if (tensors[i] == parent) return invalid("the parents cannot be a state");
         for (int j = 0; j < i; j++)
             if (tensors[i] == tensors[j]) return invalid("a state is given twice");
     }

@@ -305,7 +305,7 @@ DLLM_API dllm_status dllm_cuda_lmhead_logits_i8(int rows, int hidden, int vocab,
  *     and L = max(lengths[b], 1); its logits are not read.
  *   - A row with an unmasked NaN or +inf, or a score of NaN or +inf, offers nothing; its status
  *     word gets DLLM_ROW_ERR_NONFINITE.
- * beams <= DLLM_BEAM_MAX, k <= DLLM_BEAM_K_MAX.  Outputs may be the arrays of the inputs of the
+ * beams <= DLLM_BEAM_MAX, k <= DLLM_BEAM_K_MAX, vocab <= 2^30.  Outputs may be the arrays of the inputs of the
  * same shape (k = beams).
  *
  * dllm_cuda_beam_reorder: state[s][b] = state[s][parent[s][b]] for each of `ntensors` tensors, in

@@ -203,6 +203,37 @@ def test_select_orders_of_values(kind, k):
     check(capi.beam_select(x, sc, k), reference(x, sc, k)[0], k)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("value", ["lowest", "highest", -1e6, 2.0 ** 20, 3e4])
+def test_select_log_probabilities_of_huge_logits(dtype, value):
+    """equal logits have the probability 1 / n, however large they are"""
+    V = 5000
+    v = {"lowest": torch.finfo(dtype).min, "highest": torch.finfo(dtype).max}.get(value, value)
+    if abs(v) > torch.finfo(dtype).max:
+        pytest.skip("not a number of this type")
+    x = torch.full((2, V), v, dtype=dtype, device=DEV)
+    allow = np.zeros((2, V), bool)
+    allow[:, 7:4000:31] = True
+    mask = torch.from_numpy(pack_mask(allow).view(np.int32)).to(DEV)
+    for kw, n, ids in ((dict(), V, [0, 1, 2]), (dict(mask=mask), int(allow[0].sum()), [7, 38, 69])):
+        got = capi.beam_select(x, torch.tensor([[-1.0, -1.5]], device=DEV), 3, **kw)
+        assert got[1].tolist() == [[0, 0, 0]] and got[2].tolist() == [ids]
+        assert (got[0].double().cpu() + 1 + np.log(n)).abs().max() <= TOL + 2.0 ** -24 * 11
+
+
+@pytest.mark.parametrize("alpha", [1000.0, -1000.0, 40.0])
+def test_select_extreme_length_penalty(alpha):
+    """ranks stay finite: the choice is defined, and every slot is filled once"""
+    rng = np.random.default_rng(3)
+    x, sc = rows(rng, 8, 4000, torch.float32), beam_scores(rng, 2, 4)
+    sc[0, 0] = 0.0
+    ln = torch.tensor([[1, 50, 100000, 7], [0, 0, 3, 3]], dtype=torch.int32, device=DEV)
+    score, parent, token = capi.beam_select(x, sc, 6, lengths=ln, length_penalty=alpha)
+    assert (parent >= 0).all() and torch.isfinite(score).all()
+    for s in range(2):
+        assert len({(int(p), int(t)) for p, t in zip(parent[s], token[s])}) == 6
+
+
 def test_select_nonfinite_rows_and_scores():
     rng = np.random.default_rng(5)
     x, sc = rows(rng, 8, 9000, torch.float32), beam_scores(rng, 2, 4)
@@ -395,6 +426,19 @@ def test_reorder_cache_views(dtype, length, dim):
     assert all(torch.equal(a, b) for a, b in zip(full, want))
 
 
+@pytest.mark.parametrize("dtype,length", [(torch.bfloat16, 101), (torch.bfloat16, 7), (torch.float32, 99), (torch.uint8, 1),
+                                          (torch.uint8, 4099)])
+def test_reorder_short_last_vector(dtype, length):
+    """runs that start on multiples of 16 bytes and end between them: what follows a run stays as it was"""
+    rng = np.random.default_rng(length)
+    p = parents_of(rng, 3, 6, "random")
+    full = torch.randint(0, 100, (18, 2, 8192), device=DEV).to(dtype)
+    want = full.clone()
+    want[:, :, :length] = moved(full[:, :, :length], p)
+    capi.beam_reorder([full[:, :, :length]], p)
+    assert torch.equal(full, want)
+
+
 def test_reorder_other_layouts():
     rng = np.random.default_rng(1)
     B, K = 3, 4
@@ -456,6 +500,7 @@ def test_reorder_refusals():
         lambda: capi.beam_reorder([t], p.cpu()),
         lambda: capi.beam_reorder([t], p.t()),
         lambda: capi.beam_reorder([t, t], p),
+        lambda: capi.beam_reorder([p.view(8, 1)], p),
         lambda: capi.beam_reorder([t, t[:, :10]], p),
         lambda: capi.beam_reorder([torch.zeros(1, 30, device=DEV).expand(8, 30)], p),
         lambda: capi.beam_reorder([torch.zeros(8, 1, device=DEV).expand(8, 30)], p),
@@ -514,6 +559,7 @@ def test_stream_argument():
     assert torch.equal(q, q2) and torch.equal(m, capi.matmul_i8(q2, scale2, q2, scale2))
     assert torch.equal(lg, capi.lmhead_logits_i8(t, q2, scale2))
     assert torch.equal(capi.beam_select(x, sc, 4, stream=0)[2], want[2])
+    assert torch.equal(capi.beam_select(logits=x, scores=sc, k=4, stream=s.cuda_stream)[2], want[2])
 
 
 def test_calls_from_several_threads():

@@ -87,7 +87,8 @@ def _beam(**kw):
 @pytest.mark.parametrize("kw,rc", [
     (dict(batch=0), OK), (dict(batch=0, logits=None, scores=None), OK),
     (dict(batch=-1), INVALID), (dict(beams=0), INVALID), (dict(vocab=0), INVALID), (dict(k=0), INVALID),
-    (dict(beams=129), UNSUPPORTED), (dict(k=257), UNSUPPORTED), (dict(dtype=4), INVALID), (dict(row_stride=99), INVALID),
+    (dict(beams=129), UNSUPPORTED), (dict(k=257), UNSUPPORTED),
+    (dict(vocab=2 ** 30 + 1, row_stride=2 ** 31), UNSUPPORTED), (dict(dtype=4), INVALID), (dict(row_stride=99), INVALID),
     (dict(logits=None), INVALID), (dict(scores=None), INVALID), (dict(out_score=None), INVALID),
     (dict(out_parent=None), INVALID), (dict(out_token=None), INVALID), (dict(logits=P + 2), INVALID),
     (dict(logits=P + 1, dtype=1), INVALID), (dict(mask=P, mask_stride=3), INVALID), (dict(finished=P), INVALID),
@@ -107,7 +108,7 @@ def test_beam_select_needs_a_descriptor():
     assert lib.dllm_cuda_beam_workspace_bytes(C.byref(_beam())) > 0
 
 
-def _reorder(ptrs=(P,), **kw):
+def _reorder(ptrs=(3 * P,), **kw):
     a = dict(batch=2, beams=4, parent=P, n=len(ptrs), tensors=(C.c_void_p * max(len(ptrs), 1))(*ptrs), row_stride=64,
              segs=1, seg_stride=0, run=64)
     a.update(kw)
@@ -118,7 +119,8 @@ def _reorder(ptrs=(P,), **kw):
     (dict(batch=0), OK), (dict(ptrs=()), OK), (dict(segs=0), OK), (dict(run=0), OK),
     (dict(batch=-1), INVALID), (dict(beams=0), INVALID), (dict(n=-1), INVALID), (dict(segs=-1), INVALID),
     (dict(run=-1), INVALID), (dict(beams=129), UNSUPPORTED), (dict(parent=None), INVALID), (dict(tensors=None), INVALID),
-    (dict(ptrs=(P, None)), INVALID), (dict(ptrs=(P, 2 * P, P)), INVALID),           # twice the same state
+    (dict(ptrs=(3 * P, None)), INVALID), (dict(ptrs=(3 * P, 2 * P, 3 * P)), INVALID),           # twice the same state
+    (dict(ptrs=(2 * P,), parent=2 * P), INVALID),
     (dict(row_stride=63), INVALID), (dict(row_stride=0), INVALID), (dict(row_stride=-64), INVALID),
     (dict(segs=3, seg_stride=63), INVALID), (dict(segs=3, seg_stride=64, row_stride=128), INVALID),  # runs overlap
     (dict(segs=3, seg_stride=0, row_stride=192), INVALID),                            # a broadcast state
