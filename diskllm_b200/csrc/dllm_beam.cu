@@ -7,6 +7,15 @@
 // Within a beam that order is the order of the logits, so a row is read once: a piece of it keeps
 // its k best (logit desc, id asc) and its running maximum and exponential sum, and one CTA per
 // sequence joins the pieces.
+//
+// Measured on B200 (GPU time of a call, several back to back):
+//   64 x 8 rows of 262144 in bf16, k = 16    76 us (268 MB: 3.5 TB/s); 41 us at the measured copy rate
+//   16 x 8 rows of 151936 in fp32, 2 % allowed, a quarter of the beams ended    24 us (30 MB read)
+//   8 x 4 rows of 128257 in bf16    15 us;  1 x 4 rows of 32000 in fp32    9 us
+// What bounds the first: per tile 32 exponentials of each lane on the special-function unit (58 % busy;
+// 30 us of it alone) and the instructions around them (60 % of the issue slots), with 24 warps per SM;
+// without any candidates the pass takes 57 us.  The last two are launch and dependency latency: two
+// kernels, the second launched while the first runs.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -631,7 +640,8 @@ __device__ __forceinline__ void masked_piece(const dllm_beam_desc &d, PieceShare
     c.finish(sum, out);
 }
 
-// Persistent, 3 or 4 CTAs per SM: each takes its share of the tiles, piece by piece.
+// Persistent, 3 or 4 CTAs per SM: each takes its share of the tiles, piece by piece.  (A CTA per row left
+// the SMs with 4 and with 3 rows: 512 rows took as long as 592.)
 template <int DT, bool MASK>
 __global__ void __launch_bounds__(BS_NT, MASK ? 4 : 3) beam_pieces_kernel(dllm_beam_desc d, Split split, PieceSum *sums,
                                                                           uint64_t *cands) {
@@ -667,7 +677,8 @@ __device__ __forceinline__ bool before(const Best &a, const Best &b) {
     return a.comp > b.comp;
 }
 
-// One CTA per sequence: the beams' log-sum-exps from their pieces, then the k best of the pieces'
+// One CTA per sequence (6 to 8 us, of which most is the latency of its five dependent phases): the beams'
+// log-sum-exps from their pieces, then the k best of the pieces'
 // candidates.  The same threshold as in a piece (over the threads' best ranks, rounded down to
 // fp32, which keeps their order) leaves a few; each one's place is the number that comes before
 // it.  Where more are left than fit, the threshold is raised to the highest that k candidates
@@ -945,7 +956,8 @@ struct ReorderArgs {
     int64_t row_stride, seg_stride, run;  // bytes
 };
 
-// A CTA owns one column range (one vector per thread) of one segment for all beams of a sequence:
+// 16 caches of 64 rows, 5 of 8 beams moved: 384 us for 2.3 GB (6.0 TB/s, 0.92 of the measured copy rate),
+// bound by HBM.  A CTA owns one column range (one vector per thread) of one segment for all beams of a sequence:
 // every thread first copies the vectors that others need into its own shared-memory column, then
 // writes them out, so no second buffer is needed and beams that stay are neither read nor written.
 template <int VB>
