@@ -700,6 +700,7 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
     __shared__ Best wbest[BS_WARPS];
     __shared__ uint64_t left_key[BM_LEFT], left_comp[BM_LEFT];
     __shared__ int left_beam[BM_LEFT];
+    __shared__ float left_score[BM_LEFT];
     __shared__ Tops tops;
     __shared__ int wnumber[BS_WARPS];
     __shared__ int nleft;
@@ -800,13 +801,10 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
         const int b = e / per_beam;
         return candidate_of(e, b, comp_at(e, b), c);
     };
-    auto emit = [&](int place, const Best &c, bool none) {
-        float score = -INFINITY;
-        if (!none) {
-            double cum = (double)score_in[c.beam];
-            if (live[c.beam] == 1) cum += log_prob(c.beam, c.comp);
-            score = __double2float_rn(cum);
-        }
+    auto score_of = [&](int b, uint64_t comp) {
+        return __double2float_rn(live[b] == 1 ? (double)score_in[b] + log_prob(b, comp) : (double)score_in[b]);
+    };
+    auto emit = [&](int place, const Best &c, float score, bool none) {
         d.out_score[item * k + place] = score;
         d.out_parent[item * k + place] = none ? -1 : c.beam;
         const int32_t token = none ? -1 : (int32_t)~(uint32_t)c.comp;
@@ -819,6 +817,7 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
         left_key[at] = okey64(c.rank);
         left_beam[at] = c.beam;
         left_comp[at] = c.comp;
+        left_score[at] = score_of(c.beam, c.comp);
     };
     uint32_t mx = 0, key[BM_HELD];
 #pragma unroll
@@ -882,23 +881,24 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
         n = nleft;
     }
     if (n <= BM_LEFT) {
-        for (int i = tid; i < n; i += BS_NT) {
-            const uint64_t key = left_key[i], comp = left_comp[i];
-            const int beam = left_beam[i];
-            int place = 0, same = 0;
-#pragma unroll 4
-            for (int j = 0; j < n; j++) {
-                const uint64_t other = left_key[j];
-                place += other > key;
-                same += other == key;
+        for (int i0 = 0; i0 < n; i0 += BS_NT / 8) {  // eight lanes compare one with all
+            const int i = i0 + tid / 8;
+            const int mine_at = i < n ? i : 0, beam = left_beam[mine_at];
+            const uint64_t key = left_key[mine_at], comp = left_comp[mine_at];
+            int place = 0;
+#pragma unroll 2
+            for (int j = tid % 8; j < n; j += 8) {  // no branches: equal ranks are common in 16-bit logits
+                const uint64_t other = left_key[j], other_comp = left_comp[j];
+                const int other_beam = left_beam[j];
+                const bool earlier = (other_beam < beam) | ((other_beam == beam) & (other_comp > comp));
+                place += (other > key) | ((other == key) & earlier);
             }
-            if (same > 1)
-                for (int j = 0; j < n; j++)
-                    if (left_key[j] == key)
-                        place += left_beam[j] < beam || (left_beam[j] == beam && left_comp[j] > comp);
-            if (place < k) emit(place, Best{0.0, beam, comp}, false);
+#pragma unroll
+            for (int o = 4; o; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+            if (tid % 8 || i >= n) continue;
+            if (place < k) emit(place, Best{0.0, beam, comp}, left_score[i], false);
         }
-        for (int i = n + tid; i < k; i += BS_NT) emit(i, Best{}, true);
+        for (int i = n + tid; i < k; i += BS_NT) emit(i, Best{}, -INFINITY, true);
         return;
     }
     Best last = {INFINITY, -1, 0};
@@ -921,7 +921,7 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
         for (int w = 1; w < BS_WARPS; w++)
             if (before(wbest[w], best)) best = wbest[w];
         __syncthreads();
-        if (tid == 0) emit(r, best, false);  // more candidates than BM_LEFT >= k: there is one
+        if (tid == 0) emit(r, best, score_of(best.beam, best.comp), false);  // more candidates than BM_LEFT >= k: there is one
         last = best;
     }
 }
