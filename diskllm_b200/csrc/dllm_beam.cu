@@ -421,12 +421,15 @@ struct Piece {
         if (n <= BS_NT) {  // each candidate's place is the number of larger ones
             for (int i = lane; i < count; i += 32) sh.few[at + i] = mine[i];
             __syncthreads();
-            if (tid < n) {
-                const uint64_t c = sh.few[tid];
+            for (int i0 = 0; i0 < n; i0 += BS_NT / 8) {  // eight lanes compare one with all
+                const int i = i0 + tid / 8;
+                const uint64_t c = sh.few[min(i, n - 1)];
                 int place = 0;
 #pragma unroll 4
-                for (int i = 0; i < n; i++) place += sh.few[i] > c;
-                if (place < k) out[place] = c;
+                for (int j = tid % 8; j < n; j += 8) place += sh.few[j] > c;
+#pragma unroll
+                for (int o = 4; o; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+                if (tid % 8 == 0 && i < n && place < k) out[place] = c;
             }
             for (int i = n + tid; i < k; i += BS_NT) out[i] = 0;
         } else {
@@ -640,10 +643,10 @@ __device__ __forceinline__ void masked_piece(const dllm_beam_desc &d, PieceShare
     c.finish(sum, out);
 }
 
-// Persistent, 3 or 4 CTAs per SM: each takes its share of the tiles, piece by piece.  (A CTA per row left
+// Persistent, 4 CTAs per SM: each takes its share of the tiles, piece by piece.  (A CTA per row left
 // the SMs with 4 and with 3 rows: 512 rows took as long as 592.)
 template <int DT, bool MASK>
-__global__ void __launch_bounds__(BS_NT, MASK ? 4 : 3) beam_pieces_kernel(dllm_beam_desc d, Split split, PieceSum *sums,
+__global__ void __launch_bounds__(BS_NT, 4) beam_pieces_kernel(dllm_beam_desc d, Split split, PieceSum *sums,
                                                                           uint64_t *cands) {
     __shared__ PieceShared sh;
     asm volatile("griddepcontrol.launch_dependents;");
@@ -934,7 +937,7 @@ Split beam_split(const dllm_beam_desc *d) {
     if (d->mask) s.per_row = (int)((((int64_t)d->vocab + 31) / 32 + BS_NT - 1) / BS_NT);
     else s.per_row = (int)((((int64_t)d->vocab + 2 * vec - 2) / vec + BS_NT * BS_U - 1) / (BS_NT * BS_U));
     s.all = (int64_t)d->batch * d->beams * s.per_row;
-    const int64_t room = (int64_t)sm_count() * (d->mask ? 4 : 3);
+    const int64_t room = (int64_t)sm_count() * 4;
     s.ctas = (int)(s.all < room ? s.all : room);
     const int64_t share = s.all / s.ctas;  // tiles of a CTA, at least
     const int64_t most = (s.per_row + share - 2) / share + 1;
