@@ -243,12 +243,12 @@ def set_timing_events(before=None, after=None):
         raise DllmError(f"dllm_cuda_set_timing_events: {STATUS_NAMES.get(rc, rc)}")
 
 
-FAULT_NONE, FAULT_COPY_WAIT, FAULT_EXCHANGE_WAIT = 0, 1, 2
+FAULT_NONE, FAULT_COPY_WAIT, FAULT_EXCHANGE_WAIT, FAULT_PRODUCT_WAIT = 0, 1, 2, 8
 
 
 def inject_wait_timeout(site: int, polls: int = 1) -> None:
-    """Test hook: later sampling launches make one bounded wait run out (FAULT_COPY_WAIT or
-    FAULT_EXCHANGE_WAIT) after `polls` polls; FAULT_NONE switches it off."""
+    """Test hook: later sampling launches make one bounded wait run out (FAULT_COPY_WAIT,
+    FAULT_EXCHANGE_WAIT or, in the int8 product, FAULT_PRODUCT_WAIT) after `polls` polls; FAULT_NONE switches it off."""
     rc = load_library().dllm_cuda_debug_inject_wait_timeout(int(site), int(polls))
     if rc != DLLM_OK:
         raise DllmError(f"dllm_cuda_debug_inject_wait_timeout: {STATUS_NAMES.get(rc, rc)}")

@@ -298,6 +298,7 @@ struct MmArgs {
     int tmem_cols;   // allocated columns: two accumulators
     int early_b;     // a and its scales come from the kernel before, which may still run; b does not
     float softcap;
+    long long fault_polls;  // test hook: the issuing thread's first wait is for something that nothing completes
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -335,6 +336,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
             return false;
         }
     }
+}
+// Test hook: a wait for a barrier that nothing completes runs out after `polls` polls.
+__device__ __forceinline__ bool injected_wait(uint32_t bar, long long polls, volatile int *gave_up) {
+    for (long long i = 0; i < polls; i++)
+        if (mbar_try(bar, 0)) return true;
+    *gave_up = 1;
+    return false;
 }
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
     asm volatile(
@@ -536,10 +544,12 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_kernel(const __grid_c
                 load_a();
             }
             // no copy may be in flight when the CTA ends, also where a wait ran out, nor a product's arrival
+            const uint32_t oldest = step < (uint32_t)p.stages ? 0 : step - p.stages;
+            for (uint32_t i = oldest; i < step; i++)
+                if (!mbar_wait(empty + 8 * (i % p.stages), (i / p.stages) & 1, &gave_up)) break;
             volatile int alone = 0;
-            const uint32_t last = gave_up ? full : empty;
-            for (uint32_t i = step < (uint32_t)p.stages ? 0 : step - p.stages; i < step; i++)
-                mbar_wait(last + 8 * (i % p.stages), (i / p.stages) & 1, &alone);
+            for (uint32_t i = oldest; gave_up && i < step; i++)
+                mbar_wait(full + 8 * (i % p.stages), (i / p.stages) & 1, &alone);
         }
         __syncwarp();
     } else if (wid == 1) {
@@ -547,7 +557,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_kernel(const __grid_c
             // sums of signed 8-bit products in 32-bit integers, 128 rows by nt columns
             const uint32_t idesc = 2u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(p.nt >> 3) << 17 | (MM_ROWS >> 4) << 24;
             uint32_t step = 0, it = 0;
-            bool ok = true;
+            bool ok = !p.fault_polls || injected_wait(flushed, p.fault_polls, &gave_up);
             for (int64_t t = blockIdx.x; t < ntiles && ok; t += gridDim.x, it++) {
                 const uint32_t acc = it & 1;
                 if (it >= 2 && !(ok = mbar_wait(drained + 8 * acc, ((it >> 1) - 1) & 1, &gave_up))) break;
@@ -667,16 +677,19 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_split_kernel(const __
                 load_b(i);
                 load_a(i);
             }
+            const int oldest = i < p.stages ? 0 : i - p.stages;
+            for (int j = oldest; j < i; j++)
+                if (!mbar_wait(empty + 8 * (j % p.stages), (j / p.stages) & 1, &gave_up)) break;
             volatile int alone = 0;
-            const uint32_t last = gave_up ? full : empty;
-            for (int j = i < p.stages ? 0 : i - p.stages; j < i; j++)
-                mbar_wait(last + 8 * (j % p.stages), (j / p.stages) & 1, &alone);
+            for (int j = oldest; gave_up && j < i; j++)
+                mbar_wait(full + 8 * (j % p.stages), (j / p.stages) & 1, &alone);
         }
         __syncwarp();
     } else if (wid == 1) {
         if (lane == 0) {
             const uint32_t idesc = 2u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(p.nt >> 3) << 17 | (MM_ROWS >> 4) << 24;
-            for (int i = 0; i < n; i++) {
+            if (p.fault_polls) injected_wait(done, p.fault_polls, &gave_up);
+            for (int i = 0; i < n && !(p.fault_polls && gave_up); i++) {
                 const uint32_t s = i % p.stages;
                 if (!mbar_wait(full + 8 * s, (i / p.stages) & 1, &gave_up)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -838,6 +851,7 @@ dllm_status launch_matmul_i8(int m, int n, int k, const int8_t *a, int64_t lda, 
     p.k = k;
     p.softcap = softcap;
     p.early_b = early_b;
+    p.fault_polls = product_fault_polls();
     // token tiles of equal size, at most 256 (the widest instruction)
     p.token_tiles = (m + 255) / 256;
     p.nt = ((m + p.token_tiles - 1) / p.token_tiles + 15) / 16 * 16;

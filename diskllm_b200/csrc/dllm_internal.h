@@ -72,6 +72,7 @@ enum : int {
     FAULT_NONE = 0,
     FAULT_COPY_WAIT = 1,      // CTA 0, after its slice's bulk copy landed
     FAULT_EXCHANGE_WAIT = 2,  // the last CTA, after exchange #1 completed
+    FAULT_PRODUCT_WAIT = 8,   // int8 product kernels: each CTA's issuing thread, before its first product
 };
 
 // Multiprocessors of the current device, asked for once per device.
@@ -135,6 +136,7 @@ dllm_status set_debug_counters(unsigned long long *dev_counters);
 unsigned long long *debug_counters();  // the device array set by set_debug_counters, or null
 dllm_status set_timing_events(cudaEvent_t before, cudaEvent_t after);
 dllm_status set_fault_injection(int site, long long polls);
+long long product_fault_polls();
 size_t shard_part_bytes(int rows, int vlocal, int k);
 size_t sorted_ws_bytes(int rows, int vocab);
 size_t largek_ws_bytes(int rows, int vocab);

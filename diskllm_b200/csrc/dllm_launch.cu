@@ -91,11 +91,16 @@ static int dbg_rank_env() {
 static int g_fault_site = FAULT_NONE;
 static long long g_fault_limit = WAIT_LIMIT;
 
+static long long g_product_polls = 0;  // FAULT_PRODUCT_WAIT: polls before its wait gives up, 0 = off
+
+long long product_fault_polls() { return g_product_polls; }
+
 dllm_status set_fault_injection(int site, long long polls) {
-    if (site < FAULT_NONE || site > FAULT_EXCHANGE_WAIT || (site != FAULT_NONE && polls < 1))
-        return DLLM_ERR_INVALID_ARG;
-    g_fault_site = site;
-    g_fault_limit = site == FAULT_NONE ? WAIT_LIMIT : polls;
+    if ((site < FAULT_NONE || site > FAULT_EXCHANGE_WAIT) && site != FAULT_PRODUCT_WAIT) return DLLM_ERR_INVALID_ARG;
+    if (site != FAULT_NONE && polls < 1) return DLLM_ERR_INVALID_ARG;
+    g_product_polls = site == FAULT_PRODUCT_WAIT ? polls : 0;
+    g_fault_site = site == FAULT_PRODUCT_WAIT ? FAULT_NONE : site;
+    g_fault_limit = g_fault_site == FAULT_NONE ? WAIT_LIMIT : polls;
     return DLLM_OK;
 }
 

@@ -181,7 +181,10 @@ DLLM_API dllm_status dllm_cuda_set_debug_counters(unsigned long long *device_cou
  *     (site 1: CTA 0 waits for its slice barrier's next phase after the bulk copy landed; site 2:
  *     the last CTA waits for exchange #1's next phase after the exchange completed), giving up
  *     after `polls` polls instead of about a second.  No copy or store is in flight to the waited
- *     barrier, so the kernel goes on and the row's status gets DLLM_ROW_ERR_TIMEOUT.  Site 0
+ *     barrier, so the kernel goes on and the row's status gets DLLM_ROW_ERR_TIMEOUT.  Site 8: in the
+ *     int8 product kernels, each CTA's issuing thread waits, before its first product, for a barrier
+ *     that nothing completes; the CTA gives up, waits for its copies and returns, the outputs are not
+ *     written or not meaningful, and the call's status word gets DLLM_ROW_ERR_TIMEOUT.  Site 0
  *     switches it off.
  *   dllm_cuda_debug_fail_allocations(count): the next `count` device allocations the library
  *     makes for its own buffers fail as if cudaMalloc had run out of memory, so the calls that

@@ -293,6 +293,33 @@ def test_capture_without_a_workspace_is_refused():
     assert (out == 0).all()
 
 
+@pytest.mark.parametrize("m,n,k", [(16, 4096, 4096), (300, 30000, 640), (1, 40000, 256)])
+def test_a_wait_that_runs_out_is_reported(m, n, k):
+    """the product's issuing threads wait for something that nothing completes (no copy or product is in
+    flight to it): the kernel returns within a moment with DLLM_ROW_ERR_TIMEOUT, and the next call is right"""
+    import time
+
+    rng = np.random.default_rng(m)
+    a, b = codes(rng, m, k), codes(rng, n, k)
+    sa, sb = torch.rand(m, device=DEV), torch.rand(n, device=DEV)
+    want = capi.matmul_i8(a, sa, b, sb)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    torch.cuda.synchronize()
+    capi.inject_wait_timeout(capi.FAULT_PRODUCT_WAIT, 1000)
+    try:
+        start = time.time()
+        capi.matmul_i8(a, sa, b, sb, status=status)
+        torch.cuda.synchronize()
+        assert time.time() - start < 2.0
+    finally:
+        capi.inject_wait_timeout(capi.FAULT_NONE)
+    assert status.item() == capi.ROW_ERR_TIMEOUT
+    status.zero_()
+    for _ in range(3):
+        assert torch.equal(capi.matmul_i8(a, sa, b, sb, status=status), want)
+    assert status.item() == 0
+
+
 def test_tensor_refusals():
     q = torch.zeros(4, 40, dtype=torch.int8, device=DEV)
     s = torch.ones(4, device=DEV)
