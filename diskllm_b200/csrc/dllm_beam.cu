@@ -771,7 +771,7 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
             if (S != S || M == INFINITY) {
                 st = DLLM_ROW_ERR_NONFINITE;
                 kind = 0;
-            } else if (M > -INFINITY) l = (log2(S) + (sum_base(M) - (double)M * (double)LOG2E)) * (1.0 / (double)LOG2E);
+            } else if (M > -INFINITY) l = (log2(S) + (sum_base(M) - wide(M) * (double)LOG2E)) * (1.0 / (double)LOG2E);
             else kind = 0;
         }
         __syncwarp();
@@ -784,11 +784,11 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
     }
     __syncthreads();
     auto log_prob = [&](int b, uint64_t comp) {
-        return ((double)okey_value((uint32_t)(comp >> 32)) - (double)row_max[b]) - log_sum[b];
+        return (wide(okey_value((uint32_t)(comp >> 32))) - wide(row_max[b])) - log_sum[b];
     };
     // candidate e: position e % k of a piece's list; an ended beam offers its first position only
     auto candidate_of = [&](int e, int b, uint64_t comp, Best *c) {
-        double cum = (double)score_in[b];
+        double cum = wide(score_in[b]);
         if (live[b] == 0) return false;
         if (live[b] == 2) {
             if (e != b * per_beam) return false;
@@ -805,7 +805,7 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
         return candidate_of(e, b, comp_at(e, b), c);
     };
     auto score_of = [&](int b, uint64_t comp) {
-        return __double2float_rn(live[b] == 1 ? (double)score_in[b] + log_prob(b, comp) : (double)score_in[b]);
+        return narrow(live[b] == 1 ? wide(score_in[b]) + log_prob(b, comp) : wide(score_in[b]));
     };
     auto emit = [&](int place, const Best &c, float score, bool none) {
         d.out_score[item * k + place] = score;
@@ -827,12 +827,12 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
     for (int i = 0; i < BM_HELD; i++) {
         const int e = at_e[i];
         Best c;
-        key[i] = e < N && candidate_of(e, e / per_beam, held[i], &c) ? okey(__double2float_rd(c.rank)) : 0;
+        key[i] = e < N && candidate_of(e, e / per_beam, held[i], &c) ? okey(narrow_down(c.rank)) : 0;
         mx = max(mx, key[i]);
     }
     for (int q = lane + 32 * BM_HELD; q < warp_n; q += 32) {
         Best c;
-        if (candidate(number(q), &c)) mx = max(mx, okey(__double2float_rd(c.rank)));
+        if (candidate(number(q), &c)) mx = max(mx, okey(narrow_down(c.rank)));
     }
     tops.publish(mx, k);
     __syncthreads();
@@ -846,7 +846,7 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
     }
     for (int q = lane + 32 * BM_HELD; q < warp_n; q += 32) {
         Best c;
-        if (!candidate(number(q), &c) || okey(__double2float_rd(c.rank)) < lo) continue;
+        if (!candidate(number(q), &c) || okey(narrow_down(c.rank)) < lo) continue;
         const int at = atomicAdd(&nleft, 1);
         if (at < BM_LEFT) keep(at, c);
     }
@@ -859,7 +859,7 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
             int c_mid = 0;
             for (int e = tid; e < N; e += BS_NT) {
                 Best c;
-                c_mid += candidate(e, &c) && okey(__double2float_rd(c.rank)) >= mid;
+                c_mid += candidate(e, &c) && okey(narrow_down(c.rank)) >= mid;
             }
             c_mid = __reduce_add_sync(0xffffffffu, c_mid);
             __syncthreads();
@@ -876,7 +876,7 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
         __syncthreads();
         for (int e = tid; e < N; e += BS_NT) {
             Best c;
-            if (!candidate(e, &c) || okey(__double2float_rd(c.rank)) < reached) continue;
+            if (!candidate(e, &c) || okey(narrow_down(c.rank)) < reached) continue;
             const int at = atomicAdd(&nleft, 1);
             if (at < BM_LEFT) keep(at, c);
         }

@@ -112,8 +112,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one of t
 // With norm the sum of squares, the largest |x * g| and the scale are 64-bit too.  The factors' products
 // stay inside the range of fp32 for scales from 1e-30 to 1e30 and factors up to 1e30; rows with
 // others are divided in 64 bits.
+// Without norm 64 registers, so that 1024 threads fit on an SM (32000 x 4096 bf16: 80 us, 86 with 68
+// registers); with norm they would spill.
 template <int DT, int TPR, int E, bool VECTORS, bool NORM>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) quantize_rows_kernel(QuantArgs a) {
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, NORM ? 1 : TPR == 32 ? 4 : 1024 / TPR)
+    quantize_rows_kernel(QuantArgs a) {
     constexpr int VEC = VECTORS ? Elem<DT>::VEC : 1, NV = E / VEC;
     constexpr float MAGIC = 12582912.0f;
     __shared__ double part[2][32];
@@ -143,13 +146,13 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) quantize_rows_kernel(Qu
         double ss = 0.0, big = 0.0;
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            ss = fma((double)x[e], (double)x[e], ss);
-            const double y = fabs((double)x[e] * ((double)g[e] + (double)one));
+            ss = fma(wide(x[e]), wide(x[e]), ss);
+            const double y = fabs(wide(x[e]) * (wide(g[e]) + (double)one));
             big = y <= DBL_MAX ? fmax(big, y) : INFINITY;
             g[e] = __fadd_rn(g[e], one);
             gmax = fmaxf(gmax, fabsf(g[e]));
         }
-        rs = 1.0 / sqrt(row_reduce<false, TPR>(ss, part[0]) / (double)a.cols + (double)a.eps);
+        rs = 1.0 / sqrt(row_reduce<false, TPR>(ss, part[0]) / (double)a.cols + wide(a.eps));
         big = row_reduce<true, TPR>(big, part[1]);
         s = rs <= DBL_MAX ? scale_of(big * rs) : __int_as_float(0x7fc00000);  // else a row of zeros and eps = 0
         c = s > 0.0f ? __double2float_rn(rs / (double)s) : 0.0f;
@@ -198,8 +201,8 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) quantize_rows_kernel(Qu
                 if (fabsf(about - half) > 1e-4f) continue;
                 int code = (int)low;
                 if (NORM) {
-                    const double w = a.w && at + e < a.cols ? (double)__ldg(a.w + at + e) : 0.0;
-                    const double y = (double)x[i] * rs * (w + (double)one), border = (double)half * (double)s;
+                    const double w = a.w && at + e < a.cols ? wide(__ldg(a.w + at + e)) : 0.0;
+                    const double y = wide(x[i]) * rs * (w + (double)one), border = (double)half * (double)s;
                     code += y > border || (y == border && (code & 1));
                 } else {
                     const float rest = __fmaf_rn(-half, s, x[i]);
@@ -212,8 +215,8 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) quantize_rows_kernel(Qu
 #pragma unroll 1
             for (int e = 0; e < VEC; e++) {
                 if (at + e >= a.cols) break;
-                const double w = a.w ? (double)a.w[at + e] : 0.0;
-                const double y = (double)load_elem<DT>(src, at + e) * rs * (NORM ? w + (double)one : 1.0);
+                const double w = a.w ? wide(a.w[at + e]) : 0.0;
+                const double y = wide(load_elem<DT>(src, at + e)) * rs * (NORM ? w + (double)one : 1.0);
                 dst[at + e] = s > 0.0f ? (int8_t)__double2int_rn(y / (double)s) : 0;
             }
         } else if (VEC > 1 && at + VEC <= a.cols) {
@@ -247,14 +250,14 @@ __global__ void __launch_bounds__(QZ_LONG) quantize_long_rows_kernel(QuantArgs a
     if (a.norm) {
         double ss = 0.0;
         for (int i = t; i < a.cols; i += QZ_LONG) {
-            const double v = load_elem<DT>(src, i);
+            const double v = wide(load_elem<DT>(src, i));
             ss = fma(v, v, ss);
         }
-        rs = 1.0 / sqrt(row_reduce<false, QZ_LONG>(ss, part[0]) / (double)a.cols + (double)a.eps);
+        rs = 1.0 / sqrt(row_reduce<false, QZ_LONG>(ss, part[0]) / (double)a.cols + wide(a.eps));
     }
-    auto gain = [&](int i) { return a.w ? (double)a.w[i] + (a.add_one ? 1.0 : 0.0) : 1.0; };
+    auto gain = [&](int i) { return a.w ? wide(a.w[i]) + (a.add_one ? 1.0 : 0.0) : 1.0; };
     for (int i = t; i < a.cols; i += QZ_LONG) {
-        const double y = fabs((double)load_elem<DT>(src, i) * gain(i));
+        const double y = fabs(wide(load_elem<DT>(src, i)) * gain(i));
         big = y <= DBL_MAX ? fmax(big, y) : INFINITY;
     }
     big = row_reduce<true, QZ_LONG>(big, part[1]);
@@ -262,7 +265,7 @@ __global__ void __launch_bounds__(QZ_LONG) quantize_long_rows_kernel(QuantArgs a
     const float s = scale_of(big * rs);
     if (t == 0) a.scale[row] = s;
     for (int i = t; i < a.cols; i += QZ_LONG)
-        dst[i] = s > 0.0f ? (int8_t)__double2int_rn((double)load_elem<DT>(src, i) * rs * gain(i) / (double)s) : 0;
+        dst[i] = s > 0.0f ? (int8_t)__double2int_rn(wide(load_elem<DT>(src, i)) * rs * gain(i) / (double)s) : 0;
 }
 
 // ----------------------------------------------------------------------------------------
@@ -811,7 +814,7 @@ dllm_status quantize_typed(const QuantArgs &a, cudaStream_t stream) {
         return vec ? go(quantize_rows_kernel<DT, TPR, E, true, false>, GRID, threads)          \
                    : go(quantize_rows_kernel<DT, TPR, E, false, false>, GRID, threads);        \
     } while (0)
-    const int groups = (a.rows + 7) / 8;
+    const int groups = (int)(((int64_t)a.rows + 7) / 8);
     const bool many = a.rows >= 148;
     if (a.cols <= 512) DLLM_QUANTIZE(32, 16, groups);
     if (a.cols <= 1024 && many) DLLM_QUANTIZE(32, 32, groups);

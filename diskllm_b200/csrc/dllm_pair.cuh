@@ -1,4 +1,6 @@
-// dllm_pair.cuh -- two fp32 values in a register pair, for the instructions that work on both.
+// dllm_pair.cuh -- two fp32 values in a register pair, for the instructions that work on both, and
+// conversions to and from 64 bits.  Both keep subnormal numbers, which the compiler's own operators here
+// flush to zero.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -20,17 +22,33 @@ struct Pair {
 };
 __device__ __forceinline__ Pair add2(Pair a, Pair b) {
     Pair y;
-    asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(y.v) : "l"(a.v), "l"(b.v));
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y.v) : "l"(a.v), "l"(b.v));
     return y;
 }
 __device__ __forceinline__ Pair mul2(Pair a, Pair b) {
     Pair y;
-    asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(y.v) : "l"(a.v), "l"(b.v));
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y.v) : "l"(a.v), "l"(b.v));
     return y;
 }
 __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
     Pair y;
-    asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(y.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return y;
+}
+
+__device__ __forceinline__ double wide(float x) {
+    double y;
+    asm("cvt.f64.f32 %0, %1;" : "=d"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float narrow(double x) {
+    float y;
+    asm("cvt.rn.f32.f64 %0, %1;" : "=f"(y) : "d"(x));
+    return y;
+}
+__device__ __forceinline__ float narrow_down(double x) {
+    float y;
+    asm("cvt.rm.f32.f64 %0, %1;" : "=f"(y) : "d"(x));
     return y;
 }
 

@@ -583,3 +583,14 @@ def test_calls_from_several_threads():
     for t in threads:
         t.join()
     assert not bad
+
+
+def test_subnormal_scores():
+    """scores below the smallest normal number count, and an ended beam's is copied as it is"""
+    sc = torch.from_numpy(np.ldexp(np.array([[-3.0, -2.0, -5.0, -1.0]]), -149).astype(np.float32)).to(DEV)
+    x = torch.full((4, 100), float("-inf"), device=DEV)
+    x[:, 9] = 4.0  # the only continuation, of log-probability 0
+    done = torch.tensor([[0, 1, 1, 0]], dtype=torch.uint8, device=DEV)
+    score, parent, token = capi.beam_select(x, sc, 4, finished=done, eos=3)
+    assert parent.tolist() == [[3, 1, 0, 2]] and token.tolist() == [[9, 3, 9, 3]]
+    np.testing.assert_array_equal(score.cpu().numpy(), sc.cpu().numpy()[:, [3, 1, 0, 2]])

@@ -348,3 +348,46 @@ def test_tensor_refusals():
     ):
         with pytest.raises(capi.DllmError):
             call()
+
+
+# ---- numbers below the smallest normal one --------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cols", [40, 1000, 4096, 10001, 20000])
+@pytest.mark.parametrize("eps", [0.0, 1e-40, 1e-6])
+def test_quantize_rows_of_subnormal_values(dtype, cols, eps):
+    rng = np.random.default_rng(cols)
+    bits = 22 if dtype == torch.float32 else 6  # of the subnormal numbers' 23 and 7
+    ints = rng.integers(-(1 << bits), 1 << bits, (3, cols)).astype(np.float64)
+    x = torch.from_numpy(np.ldexp(ints, -149 if dtype == torch.float32 else -133).astype(np.float32)).to(dtype).to(DEV)
+    q, s = capi.quantize_rows_i8(x, norm=True, eps=eps)
+    rq, rs = ref_quantize(x, norm=True, eps=eps)
+    assert eps == 1e-40 or (rs > 0).all()
+    np.testing.assert_array_equal(s.cpu().numpy(), rs)
+    np.testing.assert_array_equal(q.cpu().numpy(), rq)
+
+
+@pytest.mark.parametrize("cols", [16384, 40000])
+def test_quantize_subnormal_weights(cols):
+    x = torch.full((2, cols), 2.0 ** -30, device=DEV)
+    x[0, 5], x[1, 7] = 3.0, -2.0
+    w = torch.full((cols,), float(np.ldexp(8388607.0, -149)), device=DEV)
+    q, s = capi.quantize_rows_i8(x, norm=True, norm_w=w)
+    rq, rs = ref_quantize(x, norm=True, norm_w=w)
+    assert (rs > 0).all()
+    np.testing.assert_array_equal(s.cpu().numpy(), rs)
+    np.testing.assert_array_equal(q.cpu().numpy(), rq)
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 257, 33), (3, 20000, 64)])
+def test_matmul_subnormal_results(m, n, k):
+    """the products by the scales round to multiples of 2^-149, half a step each: the first's is multiplied by
+    b_scale <= 1, so the two make at most a step"""
+    rng = np.random.default_rng(n)
+    a, b = codes(rng, m, k), codes(rng, n, k)
+    sa = torch.from_numpy(np.ldexp(rng.random(m) + 0.5, -135).astype(np.float32)).to(DEV)
+    sb = torch.from_numpy(np.ldexp(rng.random(n) + 0.5, -8).astype(np.float32)).to(DEV)
+    got = capi.matmul_i8(a, sa, b, sb).cpu().double().numpy()
+    ref = ref_matmul(a, sa, b, sb)
+    assert ((np.abs(ref) < 2.0 ** -126) & (np.abs(ref) > 2.0 ** -140)).mean() > 0.9
+    assert (np.abs(got - ref) <= 3 * U * np.abs(ref) + 2.0 ** -149).all()
