@@ -9,13 +9,13 @@
 // sequence joins the pieces.
 //
 // Measured on B200 (GPU time of a call, several back to back):
-//   64 x 8 rows of 262144 in bf16, k = 16    76 us (268 MB: 3.5 TB/s); 41 us at the measured copy rate
+//   64 x 8 rows of 262144 in bf16, k = 16    75 us (268 MB: 3.6 TB/s); 41 us at the measured copy rate
 //   16 x 8 rows of 151936 in fp32, 2 % allowed, a quarter of the beams ended    24 us (30 MB read)
-//   8 x 4 rows of 128257 in bf16    15 us;  1 x 4 rows of 32000 in fp32    9 us
-// What bounds the first: per tile 32 exponentials of each lane on the special-function unit (58 % busy;
-// 30 us of it alone) and the instructions around them (60 % of the issue slots), with 24 warps per SM;
-// without any candidates the pass takes 57 us.  The last two are launch and dependency latency: two
-// kernels, the second launched while the first runs.
+//   8 x 4 rows of 128257 in bf16    13 to 15 us;  1 x 4 rows of 32000 in fp32    9 to 11 us
+// What bounds the first (65 % of the issue slots taken, the special-function unit 59 % busy, DRAM 45 %):
+// candidates take 13 us of it, published maxima 4, the second kernel 5; without the exponentials, but
+// else whole, it is no faster, and a bare read of the rows with this layout takes 47.  The last two are
+// launch and dependency latency: two kernels, the second launched while the first runs.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -647,7 +647,7 @@ __device__ __forceinline__ void masked_piece(const dllm_beam_desc &d, PieceShare
 // the SMs with 4 and with 3 rows: 512 rows took as long as 592.)
 template <int DT, bool MASK>
 __global__ void __launch_bounds__(BS_NT, 4) beam_pieces_kernel(dllm_beam_desc d, Split split, PieceSum *sums,
-                                                                          uint64_t *cands) {
+                                                               uint64_t *cands) {
     __shared__ PieceShared sh;
     asm volatile("griddepcontrol.launch_dependents;");
     int64_t at = split.begin(blockIdx.x);
@@ -680,9 +680,8 @@ __device__ __forceinline__ bool before(const Best &a, const Best &b) {
     return a.comp > b.comp;
 }
 
-// One CTA per sequence (6 to 8 us, of which most is the latency of its five dependent phases): the beams'
-// log-sum-exps from their pieces, then the k best of the pieces'
-// candidates.  The same threshold as in a piece (over the threads' best ranks, rounded down to
+// One CTA per sequence (about 5 us, most of it the latency of its five dependent phases): the beams'
+// log-sum-exps from their pieces, then the k best of the pieces' candidates.  The same threshold as in a piece (over the threads' best ranks, rounded down to
 // fp32, which keeps their order) leaves a few; each one's place is the number that comes before
 // it.  Where more are left than fit, the threshold is raised to the highest that k candidates
 // reach; where that still leaves too many (equal ranks), k rounds take the best candidate that
@@ -732,7 +731,8 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lists = split.pieces, per_beam = lists * k, N = K * per_beam;
     const uint64_t *mine = cands + item * N;
-    // The warps take the pieces' lists in turn, so that the best are spread over them.  Candidate number q of a warp is position q % k of its list q / k.
+    // The warps take the pieces' lists in turn, so that the best are spread over them.  Candidate number q
+    // of a warp is position q % k of its list q / k.
     const int warp_n = ((K * lists - wid + BS_WARPS - 1) / BS_WARPS) * k;
     auto number = [&](int q) { return q < warp_n ? ((q / k) * BS_WARPS + wid) * k + q % k : N; };
     auto comp_at = [&](int e, int b) {  // a beam that offers none, or a piece that is not there, has none

@@ -10,7 +10,7 @@
 //   product 2048 x 8192 x 8192 to bf16    106 us (2.6e15 operations/s), 123 us once the power cap holds the
 //     clock; 16 x 4096 x 4096    8.4 us
 //   LM head 1 x 4096 x 128256    86 us (526 MB: 6.1 TB/s, 0.94 of the measured copy rate);
-//     256 x 2304 x 256000 with softcap    176 us (852 MB, 130 us at the copy rate)
+//     256 x 2304 x 256000 with softcap    172 us (852 MB, 130 us at the copy rate)
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -461,7 +461,9 @@ __device__ __forceinline__ void store_tile(const MmArgs &p, uint32_t lanes, int 
 // With few tokens the stream of b bounds it (11 stages of 18 KB in flight on each SM); with 256, b and
 // the stores together (without stores 147 of 165 us); with thousands the tensor unit (73 % busy while
 // the SMs are, 86 % of the last wave of tiles filled) at the clock that the power cap leaves.  Pairs of
-// CTAs on one tile (half the traffic of a from L2) were no faster, nor was asking for b in L2 ahead.
+// CTAs on one tile (half the traffic of a from L2) were no faster, nor was asking for b in L2 ahead, nor
+// a pipeline each for a and b (7 stages of b and 4 of a at 256 tokens: 167 and 168 us, at 128 tokens 111
+// and 101).
 template <int DT, bool CAP>
 __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_kernel(const __grid_constant__ CUtensorMap map_a,
                                                                   const __grid_constant__ CUtensorMap map_b, MmArgs p) {
@@ -618,8 +620,9 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_kernel(const __grid_c
 }
 
 // The same product for few tiles (16 x 4096 x 4096: 32 tiles on 128 CTAs take 8.4 us, on 32 CTAs
-// 13.7): a cluster of CTAs per tile, each taking a part of k.  The parts' integer sums are exchanged through distributed shared memory (over the drained pipeline stages):
-// every CTA adds up and stores 128 / cluster of the tile's channels.
+// 13.7): a cluster of CTAs per tile, each taking a part of k.  The parts' integer sums are exchanged
+// through distributed shared memory (over the drained pipeline stages): every CTA adds up and stores
+// 128 / cluster of the tile's channels.
 template <int DT, bool CAP>
 __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_split_kernel(const __grid_constant__ CUtensorMap map_a,
                                                                         const __grid_constant__ CUtensorMap map_b,

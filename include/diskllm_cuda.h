@@ -314,8 +314,8 @@ DLLM_API dllm_status dllm_cuda_lmhead_logits_i8(int rows, int hidden, int vocab,
  *
  * dllm_cuda_beam_reorder: state[s][b] = state[s][parent[s][b]] for each of `ntensors` tensors, in
  * place (parent: device [batch][beams], values outside 0 .. beams - 1 leave the beam as it is).
- * `tensors` is a HOST array of device pointers, no two equal; each tensor holds batch x beams rows
- * row_stride bytes apart, a row being `segs` runs of run_bytes bytes, seg_stride bytes apart.
+ * `tensors` is a HOST array of device pointers to tensors that share no byte; each holds batch x beams
+ * rows row_stride bytes apart, a row being `segs` runs of run_bytes bytes, seg_stride bytes apart.
  * Bytes between runs are not touched.  Beams that keep their own state are neither read nor
  * written. */
 #define DLLM_BEAM_MAX   128

@@ -391,3 +391,18 @@ def test_matmul_subnormal_results(m, n, k):
     ref = ref_matmul(a, sa, b, sb)
     assert ((np.abs(ref) < 2.0 ** -126) & (np.abs(ref) > 2.0 ** -140)).mean() > 0.9
     assert (np.abs(got - ref) <= 3 * U * np.abs(ref) + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cols", [40, 1000, 4096, 20000])
+def test_quantize_subnormal_values_beside_a_normal_one(dtype, cols):
+    """the scale is just above the smallest normal number, so the subnormal values have codes of -1, 0 and 1"""
+    rng = np.random.default_rng(cols)
+    ints = rng.integers(-127, 128, (2, cols)).astype(np.float64)
+    ints[:, cols // 3] = [128 * 127.0, 128 * 129.0]
+    x = torch.from_numpy(np.ldexp(ints, -133).astype(np.float32)).to(dtype).to(DEV)
+    q, s = capi.quantize_rows_i8(x)
+    rq, rs = ref_quantize(x)
+    assert (rs > 0).all() and (np.abs(rq) == 1).any()
+    np.testing.assert_array_equal(s.cpu().numpy(), rs)
+    np.testing.assert_array_equal(q.cpu().numpy(), rq)
