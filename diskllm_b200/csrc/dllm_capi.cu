@@ -380,6 +380,9 @@ static dllm_status check_beam(const dllm_beam_desc *d) {
     if (!d->logits || !d->scores || !d->out_score || !d->out_parent || !d->out_token)
         return invalid("logits, scores and the three outputs are needed");
     if ((uintptr_t)d->logits % dtype_bytes(d->dtype) != 0) return invalid("logits are not aligned to their type");
+    if (d->k != d->beams && (d->out_score == d->scores || (d->lengths && d->out_lengths == d->lengths) ||
+                             (d->finished && d->out_finished == d->finished)))
+        return invalid("outputs over the inputs need k = beams");
     return DLLM_OK;
 }
 

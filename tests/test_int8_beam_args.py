@@ -76,7 +76,7 @@ def test_lmhead_workspace_bytes():
 
 def _beam(**kw):
     d = capi.BeamDesc()
-    a = dict(batch=2, beams=4, vocab=100, k=8, row_stride=100, dtype=0, logits=P, scores=P, eos=-1, out_score=P,
+    a = dict(batch=2, beams=4, vocab=100, k=8, row_stride=100, dtype=0, logits=P, scores=P + 4096, eos=-1, out_score=P,
              out_parent=P, out_token=P, workspace=P, workspace_bytes=1 << 24)
     a.update(kw)
     for name, v in a.items():
@@ -95,6 +95,8 @@ def _beam(**kw):
     (dict(out_finished=P), INVALID), (dict(length_penalty=1.0), INVALID), (dict(out_lengths=P), INVALID),
     (dict(length_penalty=float("nan"), lengths=P), INVALID), (dict(length_penalty=float("inf"), lengths=P), INVALID),
     (dict(workspace=P + 16), INVALID), (dict(workspace_bytes=16), INVALID),
+    # outputs of another shape over the inputs: a sequence's would lie over the next one's inputs
+    (dict(scores=P), INVALID), (dict(lengths=P, out_lengths=P), INVALID), (dict(eos=1, finished=P, out_finished=P), INVALID),
 ])
 def test_beam_select_refusals(kw, rc):
     assert capi.load_library().dllm_cuda_beam_select(C.byref(_beam(**kw)), None) == rc
