@@ -75,6 +75,7 @@ __device__ __forceinline__ Pair exp2_approx(Pair x) {
 // changes the result by that much times the softmax's entropy.
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float BASE_EXACT = 1048576.0f;
+__device__ __forceinline__ bool beyond(float m) { return fabsf(m) >= BASE_EXACT && m > -INFINITY; }
 __device__ __forceinline__ double sum_base(float m) {
     return fabsf(m) < BASE_EXACT ? (double)__fmul_rn(m, LOG2E) : (double)m * (double)LOG2E;
 }
@@ -337,10 +338,11 @@ struct Piece {
         if (count > BS_WCAP - 32) cut();
     }
     // The maximum and the reference of the sum after a tile whose largest element is `tm`; false where some
-    // lane's lies beyond the range in which sum_base is one rounded product.
+    // lane's lies beyond the range in which sum_base is one rounded product, or did before the tile: that
+    // lane's sum is relative to the exact product, of which `base` is a rounding.
     __device__ __forceinline__ bool raise(float tm) {
         const float to = max_keep(m, tm);
-        const bool plain = !__any_sync(0xffffffffu, fabsf(to) >= BASE_EXACT && to > -INFINITY);
+        const bool plain = !__any_sync(0xffffffffu, beyond(to) || beyond(m));
         if (plain) {
             if (tm > m) {
                 const float b = __fmul_rn(tm, LOG2E);
