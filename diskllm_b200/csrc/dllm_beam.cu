@@ -697,7 +697,7 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
     // log-sum-exp of a row: its maximum, and what is added to that (the sum of both would lose it where
     // logits are huge)
     __shared__ float row_max[DLLM_BEAM_MAX];
-    __shared__ double log_sum[DLLM_BEAM_MAX], inv_len[DLLM_BEAM_MAX];
+    __shared__ double log_sum[DLLM_BEAM_MAX], divisor[DLLM_BEAM_MAX], inverse[DLLM_BEAM_MAX];
     __shared__ float score_in[DLLM_BEAM_MAX];  // copies, so that the outputs may lie over the inputs
     __shared__ int length_in[DLLM_BEAM_MAX];
     __shared__ int live[DLLM_BEAM_MAX];  // 0 nothing to offer, 1 its row's continuations, 2 ended
@@ -711,6 +711,7 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const int K = d.beams, k = d.k;
     const int64_t item = blockIdx.x;
+    const bool by_length = d.length_penalty != 0.0f && d.lengths;
     if (tid == 0) nleft = 0;
     tops.clear();
     // what does not come from the pieces is read while they run
@@ -723,10 +724,11 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
         npieces[b] = split.cta_of((row + 1) * split.per_row - 1) - split.cta_of(row * split.per_row) + 1;
         length_in[b] = len_in;
         score_in[b] = sc;
-        // kept within 1e-200 and 1e200, so that ranks stay finite
-        inv_len[b] = d.length_penalty != 0.0f && d.lengths
-                         ? fmin(fmax(pow(len, -(double)d.length_penalty), 1e-200), 1e200)
-                         : 1.0;
+        // L^alpha, kept within 1e-200 and 1e200, so that ranks stay finite; L itself where alpha is 1
+        divisor[b] = !by_length                   ? 1.0
+                     : d.length_penalty == 1.0f ? len
+                                                : fmin(fmax(pow(len, (double)d.length_penalty), 1e-200), 1e200);
+        inverse[b] = 1.0 / divisor[b];
         live[b] = !(sc >= -FLT_MAX && sc <= FLT_MAX) ? 0 : ended ? 2 : 1;
     }
     __syncthreads();
@@ -799,7 +801,10 @@ __global__ void __launch_bounds__(BS_NT) beam_merge_kernel(dllm_beam_desc d, con
             if (!comp) return false;
             cum += log_prob(b, comp);
         }
-        *c = {cum * inv_len[b], b, comp};
+        // cum / divisor, correctly rounded (Markstein's step on the product by the rounded reciprocal): equal
+        // ranks go to the lowest beam
+        const double rank = cum * inverse[b];
+        *c = {fma(fma(-rank, divisor[b], cum), inverse[b], rank), b, comp};
         return true;
     };
     auto candidate = [&](int e, Best *c) {

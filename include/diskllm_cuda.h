@@ -301,7 +301,7 @@ DLLM_API dllm_status dllm_cuda_lmhead_logits_i8(int rows, int hidden, int vocab,
  * a continuation (b, i) has the score cum = scores[b] + lp(b, i) and the rank cum / L^alpha, where
  * L = lengths[b] + 1 is its length in tokens (alpha = length_penalty; without lengths or with
  * alpha = 0 the rank is the score).  Order: rank descending, then beam, then logit descending,
- * then id ascending; sums and ranks are held in 64 bits.
+ * then id ascending; sums and ranks are held in 64 bits, L^alpha within 1e-200 and 1e200.
  *   - A cleared mask bit leaves id i out, whatever its logit.  Continuations of probability 0
  *     (logit -inf, score -inf) are never chosen: slots that nothing fills get score -inf,
  *     parent -1, token -1.

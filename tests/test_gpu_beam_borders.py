@@ -1,6 +1,6 @@
 """dllm_cuda_beam_select where its kernels change how they compute: logits around +-2^20, where the reference
-of the exponential sums changes its form; and the order within a beam, which is exact whatever the scores'
-tolerance.  Tolerance and reference are those of
+of the exponential sums changes its form, and ranks that are equal only as exact quotients; and the order
+within a beam, which is exact whatever the scores' tolerance.  Tolerance and reference are those of
 test_gpu_beam."""
 from __future__ import annotations
 
@@ -78,6 +78,21 @@ def test_sums_across_the_border_in_bf16(sign):
     ref, _ = reference(x, sc, k)
     check(got, ref, k)
     check_beams(got, ref)
+
+
+@pytest.mark.parametrize("ended", [True, False])
+@pytest.mark.parametrize("beams", [2, 64, 128])
+def test_ranks_are_quotients(beams, ended):
+    """scores of -3 per token: with alpha = 1 every rank is -3 exactly, and the beams come in their order"""
+    n = torch.arange(1, beams + 1, dtype=torch.int32, device=DEV).view(1, beams)
+    x = torch.full((beams, 40), float("-inf"), device=DEV)
+    x[:, 6] = 0.0  # the only continuation; its log-probability is exactly 0
+    done = torch.full((1, beams), int(ended), dtype=torch.uint8, device=DEV)
+    sc = -3.0 * n.float()
+    score, parent, token = capi.beam_select(x, sc, beams, finished=done, eos=9, lengths=n if ended else n - 1,
+                                            length_penalty=1.0)
+    assert parent.tolist() == [list(range(beams))]
+    assert torch.equal(score, sc) and (token == (9 if ended else 6)).all()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
