@@ -91,16 +91,42 @@ static dllm_status get_config(int rows, int vocab, int dtype, int hist_max, int 
 
 // ----------------------------------------------------------------------------------------
 // library-managed workspace: one grow-only buffer per (device, stream)
+//
+// A call holds its buffer (Scratch) from the lookup until its last kernel is queued.  Without that, two
+// threads' calls on one stream could queue their kernels in turn, each reading what the other's wrote
+// there, and one could free the buffer to grow it after the other took its address.
+// cudaStreamPerThread is one handle for a stream of every thread, so its buffers go by thread too; a buffer
+// whose thread has ended goes to the next new one, which frees it first (that waits for the GPU).
 
 namespace {
 struct WsEntry {
     int dev;
     void *stream;
+    long long thread;  // of cudaStreamPerThread, else 0; -1: ended
+    bool stale;        // of an ended thread, whose kernels may still run
     void *ptr;
     size_t bytes;
+    std::mutex busy;   // guards ptr and bytes, and the launches of a call
 };
-std::mutex g_ws_mu;
-std::vector<WsEntry> g_ws;
+// never destroyed: threads may end after the library's other objects
+std::mutex &g_ws_mu = *new std::mutex;
+std::vector<WsEntry *> &g_ws = *new std::vector<WsEntry *>;
+
+struct ThreadNumber {
+    long long n;
+    ThreadNumber() {
+        static std::atomic<long long> last{0};
+        n = ++last;
+    }
+    ~ThreadNumber() {
+        std::lock_guard<std::mutex> lk(g_ws_mu);
+        for (WsEntry *w : g_ws)
+            if (w->thread == n) {
+                w->thread = -1;
+                w->stale = true;
+            }
+    }
+};
 }  // namespace
 
 // Test hook: this many of the next library allocations fail as if cudaMalloc had run out of
@@ -120,28 +146,57 @@ extern "C" dllm_status dllm_cuda_debug_fail_allocations(int count) {
     return DLLM_OK;
 }
 
-static void *internal_workspace(void *stream, size_t bytes) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
-    std::lock_guard<std::mutex> lk(g_ws_mu);
-    for (auto &w : g_ws) {
-        if (w.dev != dev || w.stream != stream) continue;
-        if (w.bytes >= bytes) return w.ptr;
-        cudaFree(w.ptr);  // waits for kernels still using the old buffer
-        w.ptr = nullptr;
-        w.bytes = 0;
-        if (lib_malloc(&w.ptr, bytes) != cudaSuccess) {
-            w.ptr = nullptr;
-            return nullptr;
+// A call's hold on the library's buffer of its (device, stream).
+class Scratch {
+  public:
+    // the buffer, of at least `bytes`; nullptr where memory ran out
+    void *acquire(void *stream, size_t bytes) {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
+        WsEntry *w = entry(dev, stream);
+        held_ = std::unique_lock<std::mutex>(w->busy);
+        if (w->bytes < bytes || w->stale) {
+            cudaFree(w->ptr);  // waits for kernels still using the old buffer
+            w->ptr = nullptr;
+            w->bytes = 0;
+            w->stale = false;
+            if (lib_malloc(&w->ptr, bytes) != cudaSuccess) {
+                w->ptr = nullptr;
+                held_.unlock();
+                return nullptr;
+            }
+            w->bytes = bytes;
         }
-        w.bytes = bytes;
-        return w.ptr;
+        return w->ptr;
     }
-    void *p = nullptr;
-    if (lib_malloc(&p, bytes) != cudaSuccess) return nullptr;
-    g_ws.push_back({dev, stream, p, bytes});
-    return p;
-}
+
+  private:
+    static WsEntry *entry(int dev, void *stream) {
+        long long thread = 0;
+        if (stream == (void *)cudaStreamPerThread) {
+            static thread_local ThreadNumber number;
+            thread = number.n;
+        }
+        std::lock_guard<std::mutex> lk(g_ws_mu);
+        WsEntry *ended = nullptr;
+        for (WsEntry *w : g_ws) {
+            if (w->dev != dev || w->stream != stream) continue;
+            if (w->thread == thread) return w;
+            if (w->thread == -1) ended = w;
+        }
+        if (ended) {
+            ended->thread = thread;
+            return ended;
+        }
+        WsEntry *w = new WsEntry{};
+        w->dev = dev;
+        w->stream = stream;
+        w->thread = thread;
+        g_ws.push_back(w);
+        return w;
+    }
+    std::unique_lock<std::mutex> held_;
+};
 
 // ----------------------------------------------------------------------------------------
 // batched entry point
@@ -209,7 +264,8 @@ extern "C" dllm_status dllm_cuda_lmhead_logits(int rows, int hidden, int vocab, 
         return DLLM_ERR_INVALID_ARG;
     if (lmh_max_rows(hidden) < 1) return DLLM_ERR_UNSUPPORTED;
     if (rows == 0) return DLLM_OK;
-    float *scratch = (float *)internal_workspace(stream, (size_t)rows * hidden * sizeof(float));
+    Scratch lib;
+    float *scratch = (float *)lib.acquire(stream, (size_t)rows * hidden * sizeof(float));
     if (!scratch) {
         set_error("lm-head scratch", cudaErrorMemoryAllocation);
         return DLLM_ERR_OOM;
@@ -237,10 +293,11 @@ static bool codes_aligned(const void *p, int64_t stride, int cols) {
     return (uintptr_t)p % 16 == 0 && stride % 16 == 0 && stride >= cols;
 }
 
-// A call's scratch: the caller's, or the library's buffer of the (device, stream).  The library's
+// A call's scratch: the caller's, or the library's buffer of the (device, stream), held by `lib`.  That one
 // may be freed and grown by a later call, which a captured graph would not see, and growing it is
 // not allowed during a capture: refused there.
-static dllm_status scratch_for(void *given, size_t given_bytes, size_t need, cudaStream_t stream, void **out) {
+static dllm_status scratch_for(void *given, size_t given_bytes, size_t need, cudaStream_t stream, Scratch &lib,
+                               void **out) {
     if (given) {
         if ((uintptr_t)given % 256 != 0) return invalid("workspace is not 256-byte aligned");
         if (given_bytes < need) return invalid("workspace is too small");
@@ -254,7 +311,7 @@ static dllm_status scratch_for(void *given, size_t given_bytes, size_t need, cud
         return DLLM_ERR_CUDA;
     }
     if (cap != cudaStreamCaptureStatusNone) return invalid("a captured call needs a workspace of the caller");
-    *out = internal_workspace((void *)stream, need);
+    *out = lib.acquire((void *)stream, need);
     if (!*out) {
         set_error("scratch", cudaErrorMemoryAllocation);
         return DLLM_ERR_OOM;
@@ -342,9 +399,10 @@ extern "C" dllm_status dllm_cuda_lmhead_logits_i8(int rows, int hidden, int voca
     if (!h || !w || !w_scale || !logits) return invalid("h, w, w_scale and logits are needed");
     if (!codes_aligned(w, w_stride, hidden)) return invalid("w: base and stride on 16 bytes, stride >= hidden");
     if (!(eps >= 0.0f)) return invalid("eps < 0");
+    Scratch lib;
     void *ws = nullptr;
     dllm_status st = scratch_for(workspace, workspace_bytes, dllm_cuda_lmhead_i8_workspace_bytes(rows, hidden),
-                                 (cudaStream_t)stream, &ws);
+                                 (cudaStream_t)stream, lib, &ws);
     if (st != DLLM_OK) return st;
     int8_t *q = (int8_t *)ws;
     float *scale = (float *)((unsigned char *)ws + ((size_t)rows * code_stride(hidden) + 255) / 256 * 256);
@@ -397,8 +455,9 @@ extern "C" dllm_status dllm_cuda_beam_select(const dllm_beam_desc *d, void *stre
     dllm_status st = check_beam(d);
     if (st != DLLM_OK) return st;
     if (d->batch == 0) return DLLM_OK;
+    Scratch lib;
     void *ws = nullptr;
-    st = scratch_for(d->workspace, d->workspace_bytes, beam_ws_bytes(d), (cudaStream_t)stream, &ws);
+    st = scratch_for(d->workspace, d->workspace_bytes, beam_ws_bytes(d), (cudaStream_t)stream, lib, &ws);
     if (st != DLLM_OK) return st;
     st = launch_beam_select(d, ws, (cudaStream_t)stream);
     if (st == DLLM_ERR_CUDA) set_error("beam selection kernel launch", cudaGetLastError());
@@ -449,7 +508,8 @@ extern "C" dllm_status dllm_cuda_shard_candidates(const dllm_batch_desc *d, int6
     if (d->flags & ~(unsigned)DLLM_MODE_PEN_TRUE_DIV) return DLLM_ERR_UNSUPPORTED;
     // per-chunk candidates of rows wider than one chunk: the grow-only internal buffer
     const size_t pb = shard_part_bytes(d->rows, d->vocab, k);
-    void *part = pb ? internal_workspace(stream, pb) : nullptr;
+    Scratch lib;
+    void *part = pb ? lib.acquire(stream, pb) : nullptr;
     if (pb && !part) {
         set_error("shard candidate scratch", cudaErrorMemoryAllocation);
         return DLLM_ERR_OOM;
@@ -635,11 +695,12 @@ extern "C" dllm_status dllm_cuda_sample_batch(const dllm_batch_desc *d, void *st
     if (st != DLLM_OK) return st;
     const int nrec = fused ? nrec_for(cfg) : 0;
     const size_t ws_need = L.total;
+    Scratch lib;
     void *ws = d->workspace;
     if (ws) {
         if (d->workspace_bytes < ws_need) return DLLM_ERR_INVALID_ARG;
     } else {
-        ws = internal_workspace(stream, ws_need);
+        ws = lib.acquire(stream, ws_need);
         if (!ws) {
             set_error("workspace allocation", cudaErrorMemoryAllocation);
             return DLLM_ERR_OOM;

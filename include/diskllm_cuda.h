@@ -116,7 +116,10 @@ typedef struct {
 
     void *workspace;          /* optional device scratch of >= dllm_cuda_workspace_bytes()
                                  bytes (256-byte aligned); NULL: the library keeps one
-                                 buffer per (device, stream) and grows it with cudaMalloc */
+                                 buffer per (device, stream) and grows it with cudaMalloc.
+                                 Several host threads may call with NULL at once, on one
+                                 stream too, and with cudaStreamPerThread each has its own
+                                 buffer.  A buffer given here serves one call at a time */
     size_t workspace_bytes;
 } dllm_batch_desc;
 
@@ -281,7 +284,7 @@ DLLM_API dllm_status dllm_cuda_lmhead_logits(int rows, int hidden, int vocab, co
  *   and their scales: the final RMSNorm and the codes of h [rows][hidden] in one kernel, then the
  *   product and the softcap, writing fp32 logits [rows][vocab].  `workspace` holds the codes
  *   (dllm_cuda_lmhead_i8_workspace_bytes, 256-byte aligned); NULL: the library's buffer of the
- *   (device, stream), which is refused while the stream is being captured. */
+ *   (device, stream), as in dllm_batch_desc, which is refused while the stream is being captured. */
 DLLM_API dllm_status dllm_cuda_quantize_rows_i8(int rows, int cols, const void *x, int64_t x_stride, int x_dtype,
                                                 int norm, const float *norm_w, float eps, int add_one, int8_t *q,
                                                 int64_t q_stride, float *scale, void *stream);
@@ -342,8 +345,8 @@ typedef struct {
     int32_t *status;          /* optional [batch][beams] out: 0 or DLLM_ROW_ERR_NONFINITE */
 
     void *workspace;          /* device scratch of dllm_cuda_beam_workspace_bytes() bytes, 256-byte
-                                 aligned; NULL: the library's buffer of the (device, stream),
-                                 refused while the stream is being captured */
+                                 aligned; NULL: the library's buffer of the (device, stream), as in
+                                 dllm_batch_desc, refused while the stream is being captured */
     size_t workspace_bytes;
 } dllm_beam_desc;
 
