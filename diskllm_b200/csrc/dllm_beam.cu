@@ -1023,11 +1023,11 @@ __global__ void __launch_bounds__(RO_NT) beam_reorder_kernel(ReorderArgs a) {
 }  // namespace
 
 template <auto Kernel>
-static void launch_pieces(const dllm_beam_desc &d, const Split &split, PieceSum *sums, uint64_t *cands,
-                          cudaStream_t stream) {
+static cudaError_t launch_pieces(const dllm_beam_desc &d, const Split &split, PieceSum *sums, uint64_t *cands,
+                                 cudaStream_t stream) {
     // room for four CTAs' buffers on an SM
-    set_once<Kernel>(cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-    Kernel<<<split.ctas, BS_NT, 0, stream>>>(d, split, sums, cands);
+    const cudaError_t e = set_once<Kernel>(cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    return e == cudaSuccess ? launch_kernel(Kernel, split.ctas, BS_NT, 0, stream, d, split, sums, cands) : e;
 }
 
 static size_t sums_bytes(int64_t pieces) { return ((size_t)pieces * sizeof(PieceSum) + 255) / 256 * 256; }
@@ -1044,11 +1044,11 @@ dllm_status launch_beam_select(const dllm_beam_desc *d, void *ws, cudaStream_t s
 #define DLLM_PIECES(DT)                                                                       \
     (d->mask ? launch_pieces<beam_pieces_kernel<DT, true>>(*d, split, sums, cands, stream)    \
              : launch_pieces<beam_pieces_kernel<DT, false>>(*d, split, sums, cands, stream))
-    if (d->dtype == DLLM_DTYPE_F32) DLLM_PIECES(DLLM_DTYPE_F32);
-    else if (d->dtype == DLLM_DTYPE_BF16) DLLM_PIECES(DLLM_DTYPE_BF16);
-    else DLLM_PIECES(DLLM_DTYPE_F16);
+    cudaError_t e = d->dtype == DLLM_DTYPE_F32    ? DLLM_PIECES(DLLM_DTYPE_F32)
+                    : d->dtype == DLLM_DTYPE_BF16 ? DLLM_PIECES(DLLM_DTYPE_BF16)
+                                                  : DLLM_PIECES(DLLM_DTYPE_F16);
 #undef DLLM_PIECES
-    if (cudaGetLastError() != cudaSuccess) return DLLM_ERR_CUDA;
+    if (e != cudaSuccess) return cuda_failed("beam selection kernel launch", e);
     // launched while the pieces run; it waits for them on the GPU
     cudaLaunchAttribute attr = {};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1059,10 +1059,8 @@ dllm_status launch_beam_select(const dllm_beam_desc *d, void *ws, cudaStream_t s
     cfg.stream = stream;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, beam_merge_kernel, *d, (const PieceSum *)sums, (const uint64_t *)cands, split) ==
-                   cudaSuccess
-               ? DLLM_OK
-               : DLLM_ERR_CUDA;
+    e = cudaLaunchKernelEx(&cfg, beam_merge_kernel, *d, (const PieceSum *)sums, (const uint64_t *)cands, split);
+    return e == cudaSuccess ? DLLM_OK : cuda_failed("beam selection kernel launch", e);
 }
 
 dllm_status launch_beam_reorder(int batch, int beams, const int32_t *parent, int ntensors, void *const *tensors,
@@ -1089,8 +1087,8 @@ dllm_status launch_beam_reorder(int batch, int beams, const int32_t *parent, int
         for (int t = 0; t < ntensors; t += group) {
             const int n = ntensors - t < group ? ntensors - t : group;
             for (int i = 0; i < n; i++) a.tensors[i] = (unsigned char *)tensors[t + i];
-            kernel<<<(unsigned)(per_tensor * n), nt, smem, stream>>>(a);
-            if (cudaGetLastError() != cudaSuccess) return DLLM_ERR_CUDA;
+            const cudaError_t e = launch_kernel(kernel, (unsigned)(per_tensor * n), nt, smem, stream, a);
+            if (e != cudaSuccess) return cuda_failed("beam reorder kernel launch", e);
         }
         return DLLM_OK;
     };
@@ -1098,7 +1096,7 @@ dllm_status launch_beam_reorder(int batch, int beams, const int32_t *parent, int
     cudaError_t e = vb == 16  ? set_once<beam_reorder_kernel<16>>(size, 131072)
                     : vb == 4 ? set_once<beam_reorder_kernel<4>>(size, 131072)
                               : set_once<beam_reorder_kernel<1>>(size, 131072);
-    if (e != cudaSuccess) return DLLM_ERR_CUDA;
+    if (e != cudaSuccess) return cuda_failed("beam reorder kernel set-up", e);
     return vb == 16 ? launch(beam_reorder_kernel<16>) : vb == 4 ? launch(beam_reorder_kernel<4>) : launch(beam_reorder_kernel<1>);
 }
 

@@ -30,6 +30,11 @@ extern "C" const char *dllm_cuda_last_error(void) { return g_last_error; }
 
 namespace dllm {
 void set_last_error_message(const char *msg) { snprintf(g_last_error, sizeof g_last_error, "%s", msg); }
+dllm_status cuda_failed(const char *what, cudaError_t e) {
+    set_error(what, e);
+    cudaGetLastError();
+    return DLLM_ERR_CUDA;
+}
 }  // namespace dllm
 
 extern "C" dllm_status dllm_cuda_set_timing_events(void *before, void *after) {
@@ -129,15 +134,20 @@ struct ThreadNumber {
 };
 }  // namespace
 
-// Test hook: this many of the next library allocations fail as if cudaMalloc had run out of
-// memory (dllm_cuda_debug_fail_allocations).
+// Test hook: this many of the next library allocations ask for more memory than there is
+// (dllm_cuda_debug_fail_allocations).
 static std::atomic<int> g_fail_allocs{0};
 
 static cudaError_t lib_malloc(void **p, size_t bytes) {
     int n = g_fail_allocs.load();
     while (n > 0)
-        if (g_fail_allocs.compare_exchange_weak(n, n - 1)) return cudaErrorMemoryAllocation;
-    return cudaMalloc(p, bytes);
+        if (g_fail_allocs.compare_exchange_weak(n, n - 1)) {
+            bytes = (size_t)1 << 60;
+            break;
+        }
+    const cudaError_t e = cudaMalloc(p, bytes);
+    if (e != cudaSuccess) cudaGetLastError();  // reported by the return value, and not again by a later call
+    return e;
 }
 
 extern "C" dllm_status dllm_cuda_debug_fail_allocations(int count) {
@@ -306,10 +316,7 @@ static dllm_status scratch_for(void *given, size_t given_bytes, size_t need, cud
     }
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     const cudaError_t e = cudaStreamIsCapturing(stream, &cap);
-    if (e != cudaSuccess) {
-        set_error("cudaStreamIsCapturing", e);
-        return DLLM_ERR_CUDA;
-    }
+    if (e != cudaSuccess) return cuda_failed("cudaStreamIsCapturing", e);
     if (cap != cudaStreamCaptureStatusNone) return invalid("a captured call needs a workspace of the caller");
     *out = lib.acquire((void *)stream, need);
     if (!*out) {
@@ -335,10 +342,8 @@ extern "C" dllm_status dllm_cuda_quantize_rows_i8(int rows, int cols, const void
     if (!codes_aligned(q, q_stride, cols)) return invalid("q: base and stride on 16 bytes, stride >= cols");
     if (!norm && (norm_w || add_one)) return invalid("norm_w and add_one belong to norm");
     if (norm && !(eps >= 0.0f)) return invalid("eps < 0");
-    const dllm_status st = launch_quantize_i8(rows, cols, x, x_stride, x_dtype, norm, norm_w, eps, add_one, q, q_stride,
-                                              scale, (cudaStream_t)stream);
-    if (st == DLLM_ERR_CUDA) set_error("int8 quantisation kernel launch", cudaGetLastError());
-    return st;
+    return launch_quantize_i8(rows, cols, x, x_stride, x_dtype, norm, norm_w, eps, add_one, q, q_stride, scale,
+                              (cudaStream_t)stream);
 }
 
 static dllm_status check_matmul_i8(int m, int n, int k, float softcap) {
@@ -355,15 +360,6 @@ static dllm_status check_matmul_i8(int m, int n, int k, float softcap) {
     return DLLM_OK;
 }
 
-static dllm_status run_matmul_i8(int m, int n, int k, const int8_t *a, int64_t lda, const float *sa, const int8_t *b,
-                                 int64_t ldb, const float *sb, float softcap, void *out, int64_t ldo, int out_dtype,
-                                 int32_t *status, bool early_b, cudaStream_t stream) {
-    const dllm_status st = launch_matmul_i8(m, n, k, a, lda, sa, b, ldb, sb, softcap, out, ldo, out_dtype, status,
-                                            early_b, stream);
-    if (st == DLLM_ERR_CUDA) set_error("int8 product kernel launch", cudaGetLastError());
-    return st;
-}
-
 extern "C" dllm_status dllm_cuda_matmul_i8(int m, int n, int k, const int8_t *a, int64_t a_stride,
                                            const float *a_scale, const int8_t *b, int64_t b_stride,
                                            const float *b_scale, float softcap, void *out, int64_t out_stride,
@@ -377,8 +373,8 @@ extern "C" dllm_status dllm_cuda_matmul_i8(int m, int n, int k, const int8_t *a,
         return invalid("a and b: base and stride on 16 bytes, stride >= k");
     if (out_stride < n) return invalid("out_stride < n");
     if ((uintptr_t)out % dtype_bytes(out_dtype) != 0) return invalid("out is not aligned to its type");
-    return run_matmul_i8(m, n, k, a, a_stride, a_scale, b, b_stride, b_scale, softcap, out, out_stride, out_dtype,
-                         status, false, (cudaStream_t)stream);
+    return launch_matmul_i8(m, n, k, a, a_stride, a_scale, b, b_stride, b_scale, softcap, out, out_stride, out_dtype,
+                            status, false, (cudaStream_t)stream);
 }
 
 static int64_t code_stride(int cols) { return ((int64_t)cols + 15) / 16 * 16; }
@@ -410,8 +406,8 @@ extern "C" dllm_status dllm_cuda_lmhead_logits_i8(int rows, int hidden, int voca
                                     code_stride(hidden), scale, stream);
     if (st != DLLM_OK) return st;
     // the product starts while the codes are made: only they, not the weights, come from the kernel before it
-    return run_matmul_i8(rows, vocab, hidden, q, code_stride(hidden), scale, w, w_stride, w_scale, softcap, logits,
-                         vocab, DLLM_DTYPE_F32, status, true, (cudaStream_t)stream);
+    return launch_matmul_i8(rows, vocab, hidden, q, code_stride(hidden), scale, w, w_stride, w_scale, softcap, logits,
+                            vocab, DLLM_DTYPE_F32, status, true, (cudaStream_t)stream);
 }
 
 // ----------------------------------------------------------------------------------------
@@ -459,10 +455,7 @@ extern "C" dllm_status dllm_cuda_beam_select(const dllm_beam_desc *d, void *stre
     void *ws = nullptr;
     st = scratch_for(d->workspace, d->workspace_bytes, beam_ws_bytes(d), (cudaStream_t)stream, lib, &ws);
     if (st != DLLM_OK) return st;
-    st = launch_beam_select(d, ws, (cudaStream_t)stream);
-    if (st == DLLM_ERR_CUDA) set_error("beam selection kernel launch", cudaGetLastError());
-    else if (st != DLLM_OK) set_last_error_message("too many rows for one call");
-    return st;
+    return launch_beam_select(d, ws, (cudaStream_t)stream);
 }
 
 extern "C" dllm_status dllm_cuda_beam_reorder(int batch, int beams, const int32_t *parent, int ntensors,
@@ -488,8 +481,7 @@ extern "C" dllm_status dllm_cuda_beam_reorder(int batch, int beams, const int32_
     }
     const dllm_status st = launch_beam_reorder(batch, beams, parent, ntensors, tensors, row_stride, segs, seg_stride,
                                                run_bytes, (cudaStream_t)stream);
-    if (st == DLLM_ERR_CUDA) set_error("beam reorder kernel launch", cudaGetLastError());
-    else if (st != DLLM_OK) set_last_error_message("state too large for one call");
+    if (st == DLLM_ERR_UNSUPPORTED) set_last_error_message("state too large for one call");
     return st;
 }
 

@@ -796,8 +796,9 @@ bool code_map(CUtensorMap *map, const int8_t *base, int rows, int cols, int64_t 
 template <auto Kernel>
 dllm_status launch_product(const cudaLaunchConfig_t &cfg, const CUtensorMap &map_a, const CUtensorMap &map_b,
                            const MmArgs &p) {
-    if (set_once<Kernel>(cudaFuncAttributeMaxDynamicSharedMemorySize, MM_SMEM) != cudaSuccess) return DLLM_ERR_CUDA;
-    return cudaLaunchKernelEx(&cfg, Kernel, map_a, map_b, p) == cudaSuccess ? DLLM_OK : DLLM_ERR_CUDA;
+    cudaError_t e = set_once<Kernel>(cudaFuncAttributeMaxDynamicSharedMemorySize, MM_SMEM);
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, Kernel, map_a, map_b, p);
+    return e == cudaSuccess ? DLLM_OK : cuda_failed("int8 product kernel launch", e);
 }
 
 // A warp per row up to 1024 columns; then a CTA, of 256 threads up to 8192 columns, and for the few
@@ -806,8 +807,8 @@ template <int DT>
 dllm_status quantize_typed(const QuantArgs &a, cudaStream_t stream) {
     const bool vec = (uintptr_t)a.x % 16 == 0 && (a.rows == 1 || a.x_stride * Elem<DT>::SIZE % 16 == 0);
     auto go = [&](auto kernel, int grid, int threads) {
-        kernel<<<grid, threads, 0, stream>>>(a);
-        return cudaGetLastError() == cudaSuccess ? DLLM_OK : DLLM_ERR_CUDA;
+        const cudaError_t e = launch_kernel(kernel, grid, threads, 0, stream, a);
+        return e == cudaSuccess ? DLLM_OK : cuda_failed("int8 quantisation kernel launch", e);
     };
 #define DLLM_QUANTIZE(TPR, E, GRID)                                                            \
     do {                                                                                       \
@@ -871,8 +872,10 @@ dllm_status launch_matmul_i8(int m, int n, int k, const int8_t *a, int64_t lda, 
     p.tmem_cols = 32;
     while (p.tmem_cols < 2 * p.nt) p.tmem_cols *= 2;
     CUtensorMap map_a, map_b;
-    if (!code_map(&map_a, a, m, k, lda, p.nt) || !code_map(&map_b, b, n, k, ldb, MM_ROWS))
+    if (!code_map(&map_a, a, m, k, lda, p.nt) || !code_map(&map_b, b, n, k, ldb, MM_ROWS)) {
+        set_last_error_message("int8 product: the driver makes no tensor map of the codes");
         return DLLM_ERR_CUDA;
+    }
     cudaLaunchAttribute attr[2] = {};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(parts > 1 ? tiles * parts : tiles < sms ? tiles : sms));

@@ -98,6 +98,22 @@ inline cudaError_t set_once(cudaFuncAttribute what, int value) {
     return e;
 }
 
+void set_last_error_message(const char *msg);
+// Records a CUDA call's error as the message of dllm_cuda_last_error, leaves none pending; DLLM_ERR_CUDA.
+dllm_status cuda_failed(const char *what, cudaError_t e);
+
+// A launch with its own error, whatever an earlier call left pending.
+template <class... P>
+inline cudaError_t launch_kernel(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream,
+                                 const P &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Launch configuration chosen by the host for one (vocab, dtype, history bound, top-k bound).
 struct LaunchCfg {
     int cluster;     // C
