@@ -94,7 +94,12 @@ class BeamLoop:
     beam per sequence.  A beam that has produced `eos` stays as it is.
 
     After a run: tokens [batch][beams][steps] int32 (best beam first; after an end the token is eos,
-    in slots that nothing filled -1), scores [batch][beams], lengths and finished."""
+    in slots that nothing filled -1), scores [batch][beams], lengths and finished; and status
+    [batch][beams] int32, DLLM_ROW_ERR_* bits of all steps: NONFINITE for a beam whose logits or score
+    were not finite, so that it offered nothing (its place in the sequence's later steps may be
+    another's), TIMEOUT for every beam where a wait of the LM head ran out.  Then the logits of a step
+    are not meaningful, and tokens are -1 and scores NaN.  A run returns before the GPU is done; check()
+    waits for it and raises where a status is not 0."""
 
     def __init__(self, hidden_ring: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, batch: int, beams: int,
                  steps: int, *, eos: int, length_penalty: float = 0.0, norm_w: torch.Tensor | None = None,
@@ -117,6 +122,7 @@ class BeamLoop:
         self.finished = buf(batch, beams, dtype=torch.uint8)
         self.parents, self.new = buf(batch, beams), buf(batch, beams)
         self.hist = buf(rows, steps)
+        self.head_status, self.step_status = buf(1), buf(steps, batch, beams)
         self.first = torch.full((batch, beams), float("-inf"), device=self.dev)
         self.first[:, 0] = 0.0
         # buffers given to every call, so that nothing is allocated inside a capture
@@ -133,19 +139,42 @@ class BeamLoop:
     def tokens(self) -> torch.Tensor:
         return self.hist.view(self.batch, self.beams, self.steps)
 
+    @property
+    def status(self) -> torch.Tensor:
+        return (self.step_status & capi.ROW_ERR_NONFINITE).sum(0).clamp_(max=capi.ROW_ERR_NONFINITE).int() | self.head_status
+
+    def check(self) -> torch.Tensor:
+        """Waits for the run and raises DllmError where a step of it failed; the tokens."""
+        status = self.status.cpu()
+        if (status & capi.ROW_ERR_TIMEOUT).any():
+            raise capi.DllmError("BeamLoop: a wait of the LM head ran out, the tokens are not valid")
+        if status.any():
+            raise capi.DllmError("BeamLoop: logits or scores that are not finite, in the sequences "
+                                 f"{status.any(1).nonzero().view(-1).tolist()}")
+        return self.tokens
+
     def _reset(self):
         self.scores.copy_(self.first)
         self.lengths.zero_()
         self.finished.zero_()
+        self.head_status.zero_()
+        self.step_status.zero_()
+
+    def _end(self):
+        """Where the LM head gave up nothing that looks like a result is left."""
+        late = self.head_status != 0
+        self.hist.masked_fill_(late, -1)
+        self.scores.masked_fill_(late, float("nan"))
 
     def _step(self, i: int):
         r = i % self.ring.shape[0]
-        capi.lmhead_logits_i8(self.ring[r], self.wq, self.w_scale, logits=self.logits, workspace=self.head_ws, **self.head)
+        capi.lmhead_logits_i8(self.ring[r], self.wq, self.w_scale, logits=self.logits, workspace=self.head_ws,
+                              status=self.head_status, **self.head)
         capi.beam_select(self.logits, self.scores, self.beams, finished=self.finished, eos=self.eos,
                          mask=None if self.mask_ring is None else self.mask_ring[r],
                          lengths=self.lengths, length_penalty=self.length_penalty,
                          out=(self.scores, self.parents, self.new), out_finished=self.finished,
-                         out_lengths=self.lengths, workspace=self.beam_ws)
+                         out_lengths=self.lengths, status=self.step_status[i], workspace=self.beam_ws)
         capi.beam_reorder([self.hist[:, :i], *self.states], self.parents)
         self.hist[:, i].copy_(self.new.view(-1))
 
@@ -154,6 +183,7 @@ class BeamLoop:
         self._reset()
         for i in range(self.steps):
             self._step(i)
+        self._end()
         return self.tokens
 
     def capture(self):
@@ -169,6 +199,7 @@ class BeamLoop:
             self._reset()
             for i in range(self.steps):
                 self._step(i)
+            self._end()
         return self
 
     def replay(self) -> torch.Tensor:
