@@ -988,6 +988,30 @@ def _runs(t):
     return strides[0] * esz, segs, seg_stride, run
 
 
+def _refuse_overlaps(groups, rows):
+    """Raises where states of two groups share a byte (the library looks at those of one group)."""
+    spans = sorted((p, p + (rows - 1) * row + (segs - 1) * seg + run, layout)
+                   for layout, ptrs in groups.items() for row, segs, seg, run in (layout,) for p in ptrs)
+    end, apart = 0, True
+    for first, last, _ in spans:
+        apart &= first >= end
+        end = max(end, last)
+    if apart:
+        return
+    for i, (a, a_end, la) in enumerate(spans):
+        for b, _, lb in spans[i + 1:]:
+            if b >= a_end:
+                break
+            if la != lb:  # one may lie in the other's gaps: run by run, in the order of their starts
+                runs = [(p + np.add.outer(np.arange(rows) * row, np.arange(segs) * seg).ravel(), run)
+                        for p, (row, segs, seg, run) in ((a, la), (b, lb))]
+                start = np.concatenate([r[0] for r in runs])
+                stop = np.concatenate([r[0] + r[1] for r in runs])
+                order = np.argsort(start, kind="stable")
+                if (stop[order][:-1] > start[order][1:]).any():
+                    raise DllmError("states overlap")
+
+
 @_on_stream
 def beam_reorder(states, parents):
     """Moves states after their beams' parents, in place (dllm_cuda_beam_reorder): every tensor of
@@ -1011,6 +1035,8 @@ def beam_reorder(states, parents):
                 raise DllmError("a state is given twice")
             seen.add(ptr)
             groups.setdefault(_runs(t), []).append(ptr)
+    if len(groups) > 1:
+        _refuse_overlaps(groups, rows)
     for (row, segs, seg, run), ptrs in groups.items():
         _call("dllm_cuda_beam_reorder", dev, batch, beams, parents.data_ptr(), len(ptrs),
               (C.c_void_p * len(ptrs))(*ptrs), row, segs, seg, run)

@@ -458,6 +458,41 @@ extern "C" dllm_status dllm_cuda_beam_select(const dllm_beam_desc *d, void *stre
     return launch_beam_select(d, ws, (cudaStream_t)stream);
 }
 
+// The bytes of a state: rows x segs runs, at one stride inside the other (no two of them overlap).
+namespace {
+struct Runs {
+    using wide = __int128;
+    wide rows, segs, rs, ss, run;
+    wide extent() const { return (rows - 1) * rs + (segs - 1) * ss + run; }
+    // whether two such states, at a and b, share a byte: some x outer + y inner is within run of b - a
+    bool meet(uintptr_t a, uintptr_t b) const {
+        const wide d = a < b ? b - a : a - b;
+        if (d >= extent()) return false;
+        const bool by_rows = segs == 1 || (rows > 1 && rs >= (segs - 1) * ss + run);
+        const wide outer = by_rows ? rs : ss, no = by_rows ? rows : segs;
+        const wide inner = by_rows ? ss : rs, ni = by_rows ? segs : rows;
+        for (wide x = no > 1 ? d / outer : 0, x1 = no > 1 ? x + 1 : 0; x <= x1 && x < no; x++) {
+            const wide rest = d - x * outer, y = ni > 1 ? (rest < 0 ? -rest : rest) / inner : 0;
+            for (wide j = y; j <= y + 1 && j < ni; j++) {
+                const wide off = rest < 0 ? rest + j * inner : rest - j * inner;
+                if (off < run && -off < run) return true;
+            }
+        }
+        return false;
+    }
+    // whether the state at a has a byte of [b, b + bytes)
+    bool touch(uintptr_t a, uintptr_t b, wide bytes) const {
+        if ((wide)a >= (wide)b + bytes || (wide)b >= (wide)a + extent()) return false;
+        for (wide r = 0; r < rows; r++)
+            for (wide g = 0; g < segs; g++) {
+                const wide at = (wide)a + r * rs + g * ss;
+                if (at < (wide)b + bytes && (wide)b < at + run) return true;
+            }
+        return false;
+    }
+};
+}  // namespace
+
 extern "C" dllm_status dllm_cuda_beam_reorder(int batch, int beams, const int32_t *parent, int ntensors,
                                               void *const *tensors, int64_t row_stride, int segs, int64_t seg_stride,
                                               int64_t run_bytes, void *stream) {
@@ -473,11 +508,15 @@ extern "C" dllm_status dllm_cuda_beam_reorder(int batch, int beams, const int32_
     bool fits = (rows == 1 || rs >= run) && (segs == 1 || ss >= run);
     if (rows > 1 && segs > 1) fits = fits && (rs >= (segs - 1) * ss + run || ss >= (rows - 1) * rs + run);
     if (!fits) return invalid("runs of a state overlap");
+    const Runs runs = {rows, segs, rs, ss, run};
     for (int i = 0; i < ntensors; i++) {
         if (!tensors[i]) return invalid("a state is NULL");
-        if (tensors[i] == parent) return invalid("the parents cannot be a state");
-        for (int j = 0; j < i; j++)
+        if (runs.touch((uintptr_t)tensors[i], (uintptr_t)parent, rows * (int)sizeof(int32_t)))
+            return invalid("the parents cannot be a state");
+        for (int j = 0; j < i; j++) {
             if (tensors[i] == tensors[j]) return invalid("a state is given twice");
+            if (runs.meet((uintptr_t)tensors[i], (uintptr_t)tensors[j])) return invalid("states overlap");
+        }
     }
     const dllm_status st = launch_beam_reorder(batch, beams, parent, ntensors, tensors, row_stride, segs, seg_stride,
                                                run_bytes, (cudaStream_t)stream);
