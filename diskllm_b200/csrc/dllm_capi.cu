@@ -5,6 +5,7 @@
 // reference's host-pointer contract: they copy the row to the device, run the same kernels
 // and copy results back.  None of them computes on the host.
 #include <cuda_runtime.h>
+#include <float.h>
 #include <stdint.h>
 #include <stdio.h>
 #include <stdlib.h>
@@ -348,7 +349,8 @@ extern "C" dllm_status dllm_cuda_quantize_rows_i8(int rows, int cols, const void
 
 static dllm_status check_matmul_i8(int m, int n, int k, float softcap) {
     if (m < 0 || n < 0 || k < 1) return invalid("m < 0, n < 0 or k < 1");
-    if (!(softcap >= 0.0f && softcap <= 3.4e38f)) return invalid("softcap is 0 or a positive number");
+    if (softcap != 0.0f && !(softcap >= FLT_MIN && softcap <= 3.4e38f))
+        return invalid("softcap is 0 or a positive number, not a subnormal one");
     if (m > (1 << 30) || n > (1 << 30)) {
         set_last_error_message("more than 2^30 rows of codes");
         return DLLM_ERR_UNSUPPORTED;

@@ -404,6 +404,13 @@ __device__ __forceinline__ float tanh_above_one(float z) {
     return copysignf(__fmaf_rn(-2.0f, r, 1.0f), z);
 }
 
+// A channel's scale over the softcap.  Above the largest number it is that number: sums of 0 stay 0, and
+// others' tanh is 1.
+__device__ __forceinline__ float over_cap(float sb, float cap) {
+    const float q = __fdiv_rn(sb, cap);
+    return fabsf(q) > FLT_MAX && fabsf(sb) <= FLT_MAX ? copysignf(FLT_MAX, q) : q;
+}
+
 // Half of a tile's 16-column groups: the warp's 32 channels, from its lanes' accumulators, scaled, capped
 // and stored.
 template <int DT, bool CAP>
@@ -595,7 +602,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_kernel(const __grid_c
             const int ch = (int)(t / p.token_tiles) * MM_ROWS + quarter * 32 + lane;
             const int t0 = (int)(t % p.token_tiles) * p.nt;
             float sb = ch < p.n ? __ldg(p.sb + ch) : 0.0f;
-            if (CAP) sb = __fdiv_rn(sb, p.softcap);
+            if (CAP) sb = over_cap(sb, p.softcap);
             if (it == 0 || p.token_tiles > 1) {
                 __syncwarp();
                 for (int i = lane; i < p.nt; i += 32) sa[i] = t0 + i < p.m ? __ldg(p.sa + t0 + i) : 0.0f;
@@ -749,7 +756,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_split_kernel(const __
             a1 += sums[(q * p.nt + col + 1) * own + c];
         }
         float sb = __ldg(p.sb + ch), v0, v1;
-        if (CAP) sb = __fdiv_rn(sb, p.softcap);
+        if (CAP) sb = over_cap(sb, p.softcap);
         const bool two = token + 1 < p.m;
         Pair v = mul2(mul2(Pair((float)a0, (float)a1), Pair(__ldg(p.sa + token), two ? __ldg(p.sa + token + 1) : 0.0f)),
                       Pair(sb, sb));

@@ -278,7 +278,8 @@ DLLM_API dllm_status dllm_cuda_lmhead_logits(int rows, int hidden, int vocab, co
  *   rows of a (tokens) and n rows of b (channels): the sum exact in 32-bit integers
  *   (k <= 131071), then two fp32 products, the softcap cap * tanhf(out / cap) when softcap > 0,
  *   and one rounding to out_dtype (fp32 / bf16 / fp16).  Codes may be -128 too.
- *   With softcap, a channel whose b_scale / softcap is below the smallest normal float counts as 0.
+ *   softcap is 0 or a normal float.  A channel whose b_scale / softcap is below the smallest normal float
+ *   counts as 0.
  *   status (optional, one device word): DLLM_ROW_ERR_TIMEOUT is ORed in if a bounded wait expired.
  * dllm_cuda_lmhead_logits_i8: dllm_cuda_lmhead_logits with int8 output weights w [vocab][w_stride]
  *   and their scales: the final RMSNorm and the codes of h [rows][hidden] in one kernel, then the
