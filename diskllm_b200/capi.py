@@ -1017,7 +1017,7 @@ def beam_reorder(states, parents):
     """Moves states after their beams' parents, in place (dllm_cuda_beam_reorder): every tensor of
     `states` [batch * beams][...] gets row (s, b) from row (s, parents[s][b]); parents int32
     [batch][beams], -1 leaves the beam as it is.  A view, such as the used part of a cache, is moved
-    without what lies around it.  No byte may belong to two of the states."""
+    without what lies around it.  States that share a byte are refused."""
     import torch
 
     dev = parents.get_device()

@@ -9,13 +9,16 @@
 // sequence joins the pieces.
 //
 // Measured on B200 (GPU time of a call, several back to back):
-//   64 x 8 rows of 262144 in bf16, k = 16    75 us (268 MB: 3.6 TB/s); 41 us at the measured copy rate
+//   64 x 8 rows of 262144 in bf16, k = 16    76 us (268 MB: 3.5 TB/s); 41 us at the measured copy rate
 //   16 x 8 rows of 151936 in fp32, 2 % allowed, a quarter of the beams ended    24 us (30 MB read)
-//   8 x 4 rows of 128257 in bf16    13 to 15 us;  1 x 4 rows of 32000 in fp32    9 to 11 us
+//   8 x 4 rows of 128257 in bf16    13 to 15 us;  1 x 4 rows of 32000 in fp32    9 to 12 us
+//   16 x 8 rows of 151936 in fp32, k = 8: all allowed without a mask 30 us, 10 % allowed 37, 30 to 60 % 63
 // What bounds the first (65 % of the issue slots taken, the special-function unit 59 % busy, DRAM 45 %):
 // candidates take 13 us of it, published maxima 4, the second kernel 5; without the exponentials, but
-// else whole, it is no faster, and a bare read of the rows with this layout takes 47.  The last two are
-// launch and dependency latency: two kernels, the second launched while the first runs.
+// else whole, it is no faster, and a bare read of the rows with this layout takes 47.
+// 8 x 4 rows: a piece is one tile, and a warp issues 1010 instructions for it, where a tile in the middle of a
+// piece takes 361: the rest is a piece's own work (first threshold, candidates, ranking), and the second
+// kernel, whose five phases depend on one another, ranks again.  1 x 4 rows: launch and dependency latency.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -966,8 +969,10 @@ struct ReorderArgs {
     int64_t row_stride, seg_stride, run;  // bytes
 };
 
-// 16 caches of 64 rows, 5 of 8 beams moved: 384 us for 2.3 GB (6.0 TB/s, 0.92 of the measured copy rate),
-// bound by HBM.  A CTA owns one column range (one vector per thread) of one segment for all beams of a sequence:
+// 16 caches of 64 rows, 5 of 8 beams moved: 384 us for 2.3 GB (6.0 TB/s, 0.92 of the measured copy rate), 390 to
+// 400 when calls follow one another for seconds; bound by HBM.  Rows that start on 4 bytes only: a quarter of
+// that size 252 us (115 on 16 bytes); on 2 or 1 bytes, moved byte by byte, 905.  Runs of 256 bytes, 64 x 1024 of
+// them in 4 states: 87 us (13 at the copy rate), 16 threads of a CTA with work.  A CTA owns one column range (one vector per thread) of one segment for all beams of a sequence:
 // every thread first copies the vectors that others need into its own shared-memory column, then
 // writes them out, so no second buffer is needed and beams that stay are neither read nor written.
 template <int VB>

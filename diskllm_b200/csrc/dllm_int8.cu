@@ -3,14 +3,19 @@
 //
 //   codes    y = x, or x * g / sqrt(mean(x^2) + eps); s = (float)(max|y| / 127); q = rint(y / s)
 //   product  out[m][n] = a_scale[m] * b_scale[n] * sum_k a[m][k] * b[n][k], the sum exact in int32
-//   softcap  cap * tanhf(out / cap) when cap > 0 (src/core/context.c:873-876)
+//   softcap  cap * tanh(out / cap) when cap > 0 (src/core/context.c:873-876)
 //
-// Measured on B200 (GPU time of a call, several back to back):
-//   codes of 32000 x 4096 bf16    78 us (393 MB: 5.0 TB/s); of 4 x 4096 fp32 with norm    4.5 us
-//   product 2048 x 8192 x 8192 to bf16    106 us (2.6e15 operations/s), 123 us once the power cap holds the
-//     clock; 16 x 4096 x 4096    8.4 us
-//   LM head 1 x 4096 x 128256    86 us (526 MB: 6.1 TB/s, 0.94 of the measured copy rate);
-//     256 x 2304 x 256000 with softcap    172 us (852 MB, 130 us at the copy rate)
+// Measured on B200 (GPU time of a call, a few dozen back to back; in brackets when calls follow one another
+// for seconds, so that the power cap lowers the SM clock from 1965 MHz):
+//   codes of 32000 x 4096, bf16    78 us (82 at 1.9 GHz; 393 MB: 5.0 TB/s); fp16 70, fp32 110;
+//     of 4 x 4096 fp32 with norm    4.5 us; of 2048 x 4096 fp32 with norm    29 us (6.4 at the copy rate): 64-bit
+//     operations, two to four for each value
+//     off the 16-byte path: 32000 x 4097 bf16, read by value and written by byte    378 us;
+//     8192 x 28672 bf16, too long for registers    583 us (108 at the copy rate)
+//   product 2048 x 8192 x 8192 to bf16    105 us (2.6e15 operations/s; 123 at 1.57 GHz);
+//     16 x 4096 x 4096    8.7 us
+//   LM head 1 x 4096 x 128256    85 to 89 us (91 at 1.87 GHz; 526 MB: 6.1 TB/s, 0.94 of the measured copy rate);
+//     256 x 2304 x 256000 with softcap    164 to 172 us (204 at 1.25 GHz; 852 MB, 130 us at the copy rate)
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -626,8 +631,8 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_kernel(const __grid_c
     }
 }
 
-// The same product for few tiles (16 x 4096 x 4096: 32 tiles on 128 CTAs take 8.4 us, on 32 CTAs
-// 13.7): a cluster of CTAs per tile, each taking a part of k.  The parts' integer sums are exchanged
+// The same product for few tiles (16 x 4096 x 4096: 32 tiles on 128 CTAs take 8.8 us, on 32 CTAs
+// 13.8): a cluster of CTAs per tile, each taking a part of k.  The parts' integer sums are exchanged
 // through distributed shared memory (over the drained pipeline stages): every CTA adds up and stores
 // 128 / cluster of the tile's channels.
 template <int DT, bool CAP>
@@ -808,8 +813,16 @@ dllm_status launch_product(const cudaLaunchConfig_t &cfg, const CUtensorMap &map
     return e == cudaSuccess ? DLLM_OK : cuda_failed("int8 product kernel launch", e);
 }
 
-// A warp per row up to 1024 columns; then a CTA, of 256 threads up to 8192 columns, and for the few
+// A warp per row up to 1024 columns; then a CTA, of 128 or 256 threads up to 8192 columns, and for the few
 // rows of a decode step (fewer than SMs) of 1024, whose threads have less to do one after another.
+// Both sides, in us (bf16 without norm; in brackets fp32 with norm):
+//   many rows, 32 values a thread against the next larger CTA: 16384 x 1024 a warp 12.9, 128 threads 26.2;
+//     16384 x 4096 128 threads 42.0, 256 84.7; 16384 x 8192 256 threads 83.7, 1024 199; 2048 x 16384 1024 threads
+//     36.8, long rows 95.4 [124, 121]
+//   one row of 4096: 1024 threads 2.07, 128 2.28 [4.64, 4.11]; 147 rows: 2.57, 3.61 [4.97, 4.94]
+//   148 rows of 4096: 128 threads 3.37, 1024 2.48 [5.04, 4.98]; 300 rows: 3.72, 4.61 [7.92, 12.1], so the limit could lie
+//     between one and two rows an SM
+//   one row of 1024 or 2048: 1024 threads 2.0, 128 with 16 values 1.8 [4.5, 2.8]
 template <int DT>
 dllm_status quantize_typed(const QuantArgs &a, cudaStream_t stream) {
     const bool vec = (uintptr_t)a.x % 16 == 0 && (a.rows == 1 || a.x_stride * Elem<DT>::SIZE % 16 == 0);
@@ -871,7 +884,13 @@ dllm_status launch_matmul_i8(int m, int n, int k, const int8_t *a, int64_t lda, 
     p.nt = ((m + p.token_tiles - 1) / p.token_tiles + 15) / 16 * 16;
     const int sms = sm_count(), kblocks = (k + MM_KB - 1) / MM_KB;
     const int64_t tiles = (int64_t)((n + MM_ROWS - 1) / MM_ROWS) * p.token_tiles;
-    // few tiles: split k over a cluster of up to 8 CTAs, while the SMs suffice and a part has 4 blocks
+    // Few tiles: split k over a cluster of up to 8 CTAs, while the SMs suffice and a part has 4 blocks.
+    // Measured with 16 tokens and k = 4096, in us with 1, 2, 4 and 8 parts: 8 tiles 13.8 11.6 8.2 6.5; 32 tiles 13.8
+    // 11.8 8.8 17.6; 74 tiles 15.0 15.3 25.4 32.6.  The rule counts SMs, not the places that GPCs have for whole
+    // clusters, so some sizes get a part count that runs in two rounds: 16 tiles in 8 parts 12.0 (in 4: 8.3), 36
+    // tiles in 4 parts 15.5 (in 2: 11.8).  It does not look at the tokens either: with 256 of them the exchange
+    // costs more than it saves at k = 1024 (32 tiles 16.5 in 2 parts, 7.8 in one) and gains at k = 14336 (25.4
+    // in 4 parts, 43.7 in one).  75 to 147 tiles are not split (86 tiles 15.2, at the copy rate 7.0).
     int parts = 1;
     while (parts < 8 && tiles * parts * 2 <= sms && kblocks >= parts * 8) parts *= 2;
     p.stages = (MM_SMEM - 1024) / ((MM_ROWS + p.nt) * MM_KB);

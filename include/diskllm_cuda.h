@@ -274,10 +274,12 @@ DLLM_API dllm_status dllm_cuda_lmhead_logits(int rows, int hidden, int vocab, co
  *   scale 0 and codes 0; a row with an infinity or a NaN has scale NaN and codes 0.  Quantises
  *   output weights (rows = vocabulary) once, and activations (rows = tokens) each step.
  *   Padding behind a row is left as it was.
- * dllm_cuda_matmul_i8: out[i][j] = a_scale[i] * b_scale[j] * sum over k of a[i][k] * b[j][k], for m
- *   rows of a (tokens) and n rows of b (channels): the sum exact in 32-bit integers
- *   (k <= 131071), then two fp32 products, the softcap cap * tanhf(out / cap) when softcap > 0,
- *   and one rounding to out_dtype (fp32 / bf16 / fp16).  Codes may be -128 too.
+ * dllm_cuda_matmul_i8: out[i][j] = (sum over k of a[i][k] * b[j][k]) * a_scale[i] * b_scale[j], for m
+ *   rows of a (tokens) and n rows of b (channels): the sum exact in 32-bit integers (k <= 131071) and
+ *   rounded to fp32, the two products in fp32 in this order (the first may overflow where scales are
+ *   near the ends of fp32's range), the softcap cap * tanh(out / cap) when softcap > 0, and one rounding
+ *   to out_dtype (fp32 / bf16 / fp16).  Before that rounding a normal result is within 10 x 2^-24 of the
+ *   exact one, relative to it.  Codes may be -128 too.
  *   softcap is 0 or a normal float.  A channel whose b_scale / softcap is below the smallest normal float
  *   counts as 0.
  *   status (optional, one device word): DLLM_ROW_ERR_TIMEOUT is ORed in if a bounded wait expired.
@@ -308,7 +310,7 @@ DLLM_API dllm_status dllm_cuda_lmhead_logits_i8(int rows, int hidden, int vocab,
  * then id ascending; sums and ranks are held in 64 bits, L^alpha within 1e-200 and 1e200.
  *   - A cleared mask bit leaves id i out, whatever its logit.  Continuations of probability 0
  *     (logit -inf, score -inf) are never chosen: slots that nothing fills get score -inf,
- *     parent -1, token -1.
+ *     parent -1, token -1.  A score below fp32's range is written as -inf too, with its parent and token.
  *   - An ended beam (finished[b] != 0) has one continuation, the token `eos` with its own score
  *     and L = max(lengths[b], 1); its logits are not read.
  *   - A row with an unmasked NaN or +inf, or a score of NaN or +inf, offers nothing; its status
@@ -318,8 +320,9 @@ DLLM_API dllm_status dllm_cuda_lmhead_logits_i8(int rows, int hidden, int vocab,
  *
  * dllm_cuda_beam_reorder: state[s][b] = state[s][parent[s][b]] for each of `ntensors` tensors, in
  * place (parent: device [batch][beams], values outside 0 .. beams - 1 leave the beam as it is).
- * `tensors` is a HOST array of device pointers to tensors that share no byte; each holds batch x beams
- * rows row_stride bytes apart, a row being `segs` runs of run_bytes bytes, seg_stride bytes apart.
+ * `tensors` is a HOST array of device pointers to tensors that share no byte with one another or with
+ * `parent` (others are refused); each holds batch x beams rows row_stride bytes apart, a row being `segs`
+ * runs of run_bytes bytes, seg_stride bytes apart.
  * Bytes between runs are not touched.  Beams that keep their own state are neither read nor
  * written. */
 #define DLLM_BEAM_MAX   128

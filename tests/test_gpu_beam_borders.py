@@ -95,6 +95,15 @@ def test_ranks_are_quotients(beams, ended):
     assert torch.equal(score, sc) and (token == (9 if ended else 6)).all()
 
 
+def test_a_score_below_the_range_of_fp32():
+    """it is chosen, after the others, and its score is -inf"""
+    x = torch.tensor([[3e38, -3e38, -float("inf")], [1.0, 1.0, 1.0]], device=DEV)
+    sc = torch.tensor([[-2.0, -5.0]], device=DEV)
+    score, parent, token = capi.beam_select(x, sc, 6)
+    assert parent.tolist() == [[0, 1, 1, 1, 0, -1]] and token.tolist() == [[0, 0, 1, 2, 1, -1]]
+    assert score[0, 0] == -2.0 and torch.isfinite(score[0, :4]).all() and (score[0, 4:] == -float("inf")).all()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("B,K,V,k,frac", [(2, 5, 8191, 10, 1.0), (1, 4, 128256, 8, 1.0), (5, 8, 50257, 16, 1.0),
                                           (1, 64, 3000, 128, 1.0), (1, 2, 151936, 256, 1.0), (3, 4, 40003, 8, 0.5),
