@@ -167,7 +167,11 @@ class Scratch {
         WsEntry *w = entry(dev, stream);
         held_ = std::unique_lock<std::mutex>(w->busy);
         if (w->bytes < bytes || w->stale) {
-            cudaFree(w->ptr);  // waits for kernels still using the old buffer
+            if (w->ptr && cudaFree(w->ptr) != cudaSuccess) {  // waits for kernels still using the old buffer
+                cudaGetLastError();  // not allowed now, as during a capture: the buffer stays
+                held_.unlock();
+                return nullptr;
+            }
             w->ptr = nullptr;
             w->bytes = 0;
             w->stale = false;

@@ -105,3 +105,34 @@ def test_a_failed_allocation_does_not_fail_the_next_call():
     torch.cuda.synchronize()
     # codes of 127 with a scale of 1 / 127 x 1 / sqrt(1 + 1e-6): 64 less 3.2e-5, and 3 roundings of 64 x 2^-24
     assert (out - 64).abs().max() < 1e-4 and best[2].tolist() == [[0, 1, 2, 3]]
+
+
+@pytest.mark.gpu
+def test_scratch_cannot_grow_during_another_streams_capture():
+    """the call is refused, and the scratch that was there serves again"""
+    dev = torch.device("cuda", 0)
+    lib, rt = capi.load_library(), C.CDLL("libcudart.so.12")
+    w, sw = torch.ones(32, 64, dtype=torch.int8, device=dev), torch.ones(32, device=dev)
+    h, out = torch.ones(2000, 64, device=dev), torch.zeros(2000, 32, device=dev)
+    stream, other = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def head(rows):
+        return lib.dllm_cuda_lmhead_logits_i8(rows, 64, 32, h.data_ptr(), None, 1e-6, 0, w.data_ptr(), 64, sw.data_ptr(), 0.0,
+                                              out.data_ptr(), None, None, 0, stream.cuda_stream)
+
+    assert head(3) == capi.DLLM_OK
+    torch.cuda.synchronize()
+    graph = C.c_void_p()
+    assert rt.cudaStreamBeginCapture(C.c_void_p(other.cuda_stream), 0) == 0
+    try:
+        assert head(2000) == capi.DLLM_ERR_OOM
+        assert head(3) == capi.DLLM_OK
+    finally:
+        rt.cudaStreamEndCapture(C.c_void_p(other.cuda_stream), C.byref(graph))
+        rt.cudaGetLastError()
+    torch.cuda.synchronize()
+    out.zero_()
+    assert head(2000) == capi.DLLM_OK
+    torch.cuda.synchronize()
+    assert (out - 64).abs().max() < 1e-4
